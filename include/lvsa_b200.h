@@ -300,6 +300,67 @@ typedef struct LvsaCopySegment {
 } LvsaCopySegment;
 int lvsa_copy_segments(const LvsaCopySegment* segs, int32_t n, int32_t row_bytes, void* stream);
 
+/* ---- norms before and after a block, with its gate and residual scale ----
+ * The elementwise steps of a transformer block around its attention or MLP
+ * (no counterpart in the reference, which leaves them to the model):
+ *
+ *   h = residual_scale * x + gate * post(y)      the join, where y.ptr is set
+ *   n = next(h) * (1 + scale) + shift            where n.ptr is set (h = x without a join)
+ *
+ * x, h [batch, seq, width] in stream_dtype, y, n in branch_dtype: the same
+ * type, or an fp32 stream with bf16 / f16 branches.  next / post: layer or RMS
+ * norm of a row, then weight and bias [width] (NULL: 1 and 0; the layer norm
+ * only has a bias); post may be LVSA_BLOCK_NORM_NONE.  gate, scale and shift
+ * are [batch, frames, width] (NULL: 1, 0 and 0), seq / frames consecutive
+ * tokens to each frame; a stride of 0 shares a vector.  fp32 arithmetic, one
+ * rounding of each output; n is of h before its rounding. */
+enum { LVSA_BLOCK_NORM_NONE = 0, LVSA_BLOCK_NORM_LAYER = 1, LVSA_BLOCK_NORM_RMS = 2 };
+#define LVSA_BLOCK_NORM_MAX_WIDTH 16384
+typedef struct LvsaRows { /* [batch, seq, width], width contiguous; element strides */
+  void* ptr;
+  int64_t stride_b, stride_t;
+} LvsaRows;
+typedef struct LvsaVectors { /* [batch, frames, width], width contiguous */
+  void* ptr;
+  int64_t stride_b, stride_f;
+  int32_t dtype, reserved;
+} LvsaVectors;
+typedef struct LvsaRowNorm {
+  int32_t kind; /* LVSA_BLOCK_NORM_* */
+  float eps;
+  int32_t weight_dtype, bias_dtype;
+  const void* weight;
+  const void* bias;
+} LvsaRowNorm;
+typedef struct LvsaBlockNorm {
+  LvsaRows x, y, h, n;
+  LvsaVectors gate, scale, shift;
+  LvsaRowNorm post, next;
+  float residual_scale;
+  int32_t stream_dtype, branch_dtype, batch, seq, frames, width;
+  float* stats;      /* [batch * seq][2] mean and 1 / deviation of next, for the backward; or NULL */
+  float* post_stats; /* the same of post */
+} LvsaBlockNorm;
+int lvsa_block_norm_fwd(const LvsaBlockNorm* args, void* stream);
+
+/* Gradients of the above.  f: the forward's arguments (h.ptr and n.ptr are not
+ * read; whether n.ptr is set says whether there is a next norm, and stats /
+ * post_stats are its outputs).  dh, dn: gradients of h and n (either may be
+ * NULL: zero).  Outputs with a NULL ptr are not written: dx, dy; dgate,
+ * dscale, dshift [batch, frames, width] contiguous in their dtype; dweight,
+ * dbias, dpost_weight, dpost_bias [width] in the parameters' dtypes.  Sums
+ * over rows are fp32 in a fixed order: the same call gives the same bits. */
+typedef struct LvsaBlockNormGrad {
+  LvsaBlockNorm f;
+  LvsaRows dh, dn, dx, dy;
+  LvsaVectors dgate, dscale, dshift;
+  void *dweight, *dbias, *dpost_weight, *dpost_bias;
+  void* workspace; /* 16-byte aligned */
+  int64_t workspace_bytes;
+} LvsaBlockNormGrad;
+int lvsa_block_norm_workspace(const LvsaBlockNormGrad* args, int64_t* bytes);
+int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
+
 /* Human-readable name of a status code. */
 const char* lvsa_status_str(int status);
 

@@ -28,7 +28,7 @@ LVSA_MAX_FRAMES = 2048
 
 EXPORTED_SYMBOLS = ("lvsa_mask_layout", "lvsa_build_mask", "lvsa_attn_fwd", "lvsa_quantize_e4m3",
                     "lvsa_attn_fwd_fp8", "lvsa_attn_fwd_fp8_noalloc", "lvsa_qk_prologue", "lvsa_copy_segments", "lvsa_out_proj", "lvsa_status_str",
-                    "lvsa_abi_version")
+                    "lvsa_abi_version", "lvsa_block_norm_fwd", "lvsa_block_norm_workspace", "lvsa_block_norm_bwd")
 LVSA_DTYPE_E4M3 = 2
 LVSA_DTYPE_F32 = 3
 LVSA_NORM_NONE, LVSA_NORM_RMS_ROW, LVSA_NORM_RMS_HEAD, LVSA_NORM_LAYER_HEAD = 0, 1, 2, 3
@@ -95,6 +95,38 @@ class LvsaQkPrologue(ctypes.Structure):
                 ("rope_offset", _i32)]
 
 
+LVSA_BLOCK_NORM_NONE, LVSA_BLOCK_NORM_LAYER, LVSA_BLOCK_NORM_RMS = 0, 1, 2
+LVSA_BLOCK_NORM_MAX_WIDTH = 16384
+
+
+class LvsaRows(ctypes.Structure):
+    _fields_ = [("ptr", _vp), ("stride_b", _i64), ("stride_t", _i64)]
+
+
+class LvsaVectors(ctypes.Structure):
+    _fields_ = [("ptr", _vp), ("stride_b", _i64), ("stride_f", _i64), ("dtype", _i32), ("reserved", _i32)]
+
+
+class LvsaRowNorm(ctypes.Structure):
+    _fields_ = [("kind", _i32), ("eps", ctypes.c_float), ("weight_dtype", _i32), ("bias_dtype", _i32),
+                ("weight", _vp), ("bias", _vp)]
+
+
+class LvsaBlockNorm(ctypes.Structure):
+    _fields_ = [("x", LvsaRows), ("y", LvsaRows), ("h", LvsaRows), ("n", LvsaRows),
+                ("gate", LvsaVectors), ("scale", LvsaVectors), ("shift", LvsaVectors),
+                ("post", LvsaRowNorm), ("next", LvsaRowNorm), ("residual_scale", ctypes.c_float),
+                ("stream_dtype", _i32), ("branch_dtype", _i32), ("batch", _i32), ("seq", _i32),
+                ("frames", _i32), ("width", _i32), ("stats", _vp), ("post_stats", _vp)]
+
+
+class LvsaBlockNormGrad(ctypes.Structure):
+    _fields_ = [("f", LvsaBlockNorm), ("dh", LvsaRows), ("dn", LvsaRows), ("dx", LvsaRows), ("dy", LvsaRows),
+                ("dgate", LvsaVectors), ("dscale", LvsaVectors), ("dshift", LvsaVectors),
+                ("dweight", _vp), ("dbias", _vp), ("dpost_weight", _vp), ("dpost_bias", _vp),
+                ("workspace", _vp), ("workspace_bytes", _i64)]
+
+
 class LvsaFp8Scales(ctypes.Structure):
     _fields_ = [(n, _vp) for n in ("q", "k", "v", "text_q", "text_k", "text_v", "v_ref")]
 
@@ -138,6 +170,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.lvsa_qk_prologue.restype = ctypes.c_int
         lib.lvsa_out_proj.argtypes = [ctypes.POINTER(LvsaOutProjArgs), _vp]
         lib.lvsa_out_proj.restype = ctypes.c_int
+        lib.lvsa_block_norm_fwd.argtypes = [ctypes.POINTER(LvsaBlockNorm), _vp]
+        lib.lvsa_block_norm_fwd.restype = ctypes.c_int
+        lib.lvsa_block_norm_workspace.argtypes = [ctypes.POINTER(LvsaBlockNormGrad), ctypes.POINTER(_i64)]
+        lib.lvsa_block_norm_workspace.restype = ctypes.c_int
+        lib.lvsa_block_norm_bwd.argtypes = [ctypes.POINTER(LvsaBlockNormGrad), _vp]
+        lib.lvsa_block_norm_bwd.restype = ctypes.c_int
         lib.lvsa_copy_segments.argtypes = [ctypes.POINTER(LvsaCopySegment), _i32, _i32, _vp]
         lib.lvsa_copy_segments.restype = ctypes.c_int
         lib.lvsa_status_str.argtypes = [ctypes.c_int]
