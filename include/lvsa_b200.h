@@ -316,6 +316,7 @@ int lvsa_copy_segments(const LvsaCopySegment* segs, int32_t n, int32_t row_bytes
  * rounding of each output; n is of h before its rounding. */
 enum { LVSA_BLOCK_NORM_NONE = 0, LVSA_BLOCK_NORM_LAYER = 1, LVSA_BLOCK_NORM_RMS = 2 };
 #define LVSA_BLOCK_NORM_MAX_WIDTH 16384
+#define LVSA_BLOCK_NORM_MAX_ROWS 2147483000 /* batch * seq */
 typedef struct LvsaRows { /* [batch, seq, width], width contiguous; element strides */
   void* ptr;
   int64_t stride_b, stride_t;

@@ -1,12 +1,12 @@
 // Norms before and after a transformer block, fused with its gate and
 // residual scale:
 //   h = a x + gate * post(y),   n = next(h) * (1 + scale) + shift.
-// With zhat the normalised row, next's weight and the modulation fold to
-// n = zhat A + B, A = w (1 + scale), B = b (1 + scale) + shift, and post's
-// weight and the gate to h = a x + yhat G1 + G0: two vectors each, held in
-// registers over the rows of a group (the tokens of a frame).
 //
-// A CTA walks consecutive rows, one at a time; a thread owns fixed columns.
+// A team of warps holds one row in registers, kElems values a thread at most
+// (one warp up to 1024 channels, so that its sums need no barrier), and walks
+// rows a grid's teams apart.  Modulation and norm weights are read again for
+// every row: they are the same few kilobytes for all rows of a frame and stay
+// in L1, where holding them in registers would halve the rows in flight.
 // Bound: HBM (x and y read once, h and n written once).
 #include <algorithm>
 #include <atomic>
@@ -16,133 +16,147 @@
 namespace lvsa {
 namespace {
 
-template <typename TS, typename TB, bool JOIN, bool NEXT, int VEC, int K>
-__global__ void __launch_bounds__(32 * kMaxWarps)
-    block_norm_fwd_kernel(const __grid_constant__ LvsaBlockNorm a, int64_t rows, int64_t group_rows) {
-  __shared__ float2 slots[2][kMaxWarps];
-  RowSums sums(slots);
-  const Columns<VEC, K> col(a.width);
-  const float n_mine = Columns<VEC, K>::of_warp(sums.warp, a.width);
-  const float n_lane = sums.lane < sums.warps ? Columns<VEC, K>::of_warp(sums.lane, a.width) : 0.f;
-  const int64_t r0 = first_row(rows, blockIdx.x, gridDim.x), r1 = first_row(rows, blockIdx.x + 1, gridDim.x);
+constexpr int kElems = 32;
 
-  float A[NEXT ? K : 1][VEC], B[NEXT ? K : 1][VEC], G1[JOIN ? K : 1][VEC], G0[JOIN ? K : 1][VEC];
-  int64_t group = -1;
-  for (int64_t row = r0; row < r1; ++row) {
-    const int64_t b = row / a.seq, t = row - b * a.seq;
-    if (row / group_rows != group) {
-      group = row / group_rows;
-      const int64_t f = group - b * a.frames;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!col.in[k]) continue;
-        if constexpr (NEXT) {
-          float w[VEC], bias[VEC], sc[VEC], sh[VEC];
-          any_load<VEC>(a.next.weight, a.next.weight_dtype, col.at[k], 1.f, w);
-          any_load<VEC>(a.next.bias, a.next.bias_dtype, col.at[k], 0.f, bias);
-          any_load<VEC>(a.scale.ptr, a.scale.dtype, b * a.scale.stride_b + f * a.scale.stride_f + col.at[k], 0.f, sc);
-          any_load<VEC>(a.shift.ptr, a.shift.dtype, b * a.shift.stride_b + f * a.shift.stride_f + col.at[k], 0.f, sh);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            A[k][e] = w[e] * (1.f + sc[e]);
-            B[k][e] = bias[e] * (1.f + sc[e]) + sh[e];
-          }
-        }
-        if constexpr (JOIN) {
-          float w[VEC], bias[VEC], g[VEC];
-          any_load<VEC>(a.post.weight, a.post.weight_dtype, col.at[k], 1.f, w);
-          any_load<VEC>(a.post.bias, a.post.bias_dtype, col.at[k], 0.f, bias);
-          any_load<VEC>(a.gate.ptr, a.gate.dtype, b * a.gate.stride_b + f * a.gate.stride_f + col.at[k], 1.f, g);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            G1[k][e] = g[e] * w[e];
-            G0[k][e] = g[e] * bias[e];
-          }
-        }
-      }
-    }
+struct FwdParams {
+  LvsaRows x, y, h, n;
+  Vectors v;
+  FastDiv by_seq, by_group;  // row -> sequence; row -> group (frame of a sequence)
+  uint32_t rows, frames;
+  int32_t width, warps, kind, post_kind;
+  float alpha, eps, post_eps;
+  float2 *stats, *post_stats;
+};
+
+// Warps of a CTA at most: kElems values a thread hold the widest row in 16.
+template <int VEC>
+constexpr int kWarps = VEC == 1 ? kMaxWarps : 16;
+
+template <typename TS, typename TB, bool JOIN, int VEC, int K>
+__global__ void __launch_bounds__(32 * kWarps<VEC>) block_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
+  __shared__ float2 slots[2 * kMaxWarps];
+  Team team(slots, p.warps);
+  const Columns<VEC, K> col(team, p.width);
+  const float n_mine = col.of_warp(team.warp), n_lane = team.lane < team.count ? col.of_warp(team.lane) : 0.f;
+  const uint32_t teams = blockDim.x / (32 * p.warps);
+  const bool next = !JOIN || p.n.ptr;
+
+  for (uint32_t row = blockIdx.x * teams + team.barrier - 1; row < p.rows; row += gridDim.x * teams) {
+    const uint32_t b = p.by_seq.div(row);
+    const int64_t t = row - b * p.by_seq.d, f = p.by_group.div(row) - b * p.frames;
     float z[K][VEC];
-    const TS* x = static_cast<const TS*>(a.x.ptr) + b * a.x.stride_b + t * a.x.stride_t;
+    const TS* x = static_cast<const TS*>(p.x.ptr) + b * p.x.stride_b + t * p.x.stride_t;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      Pack<TS, VEC> q;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) z[k][e] = 0.f;
-      if (col.in[k]) {
-        q.load(x + col.at[k]);
+    for (int k = 0; k < K; ++k)
+      if (col.in(k)) {
+        Pack<TS, VEC> q;
+        q.load(x + col.at(k));
         q.get(z[k]);
       }
-    }
     if constexpr (JOIN) {
       float y[K][VEC];
-      const TB* yp = static_cast<const TB*>(a.y.ptr) + b * a.y.stride_b + t * a.y.stride_t;
+      const TB* yp = static_cast<const TB*>(p.y.ptr) + b * p.y.stride_b + t * p.y.stride_t;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        Pack<TB, VEC> q;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) y[k][e] = 0.f;
-        if (col.in[k]) {
-          q.load(yp + col.at[k]);
+      for (int k = 0; k < K; ++k)
+        if (col.in(k)) {
+          Pack<TB, VEC> q;
+          q.load(yp + col.at(k));
           q.get(y[k]);
         }
-      }
-      float2 st = make_float2(0.f, 1.f);
-      if (a.post.kind != LVSA_BLOCK_NORM_NONE) {
-        st = row_stats<VEC, K>(y, col, a.post.kind, a.width, a.post.eps, n_mine, n_lane, sums);
-        if (a.post_stats && threadIdx.x == 0) reinterpret_cast<float2*>(a.post_stats)[row] = st;
-      }
-      TS* h = static_cast<TS*>(a.h.ptr) + b * a.h.stride_b + t * a.h.stride_t;
+      if (p.post_kind != LVSA_BLOCK_NORM_NONE) {
+        const float2 st = row_stats<VEC, K>(y, col, p.post_kind, p.post_eps, n_mine, n_lane, team);
+        if (p.post_stats && team.warp == 0 && team.lane == 0) p.post_stats[row] = st;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!col.in[k]) continue;
+        for (int k = 0; k < K; ++k)
+          if (col.in(k)) {
+            float w[VEC], o[VEC];
+            vector_or<VEC>(p.v.post_weight, 0, 0, col.at(k), 1.f, w);
+            vector_or<VEC>(p.v.post_bias, 0, 0, col.at(k), 0.f, o);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          z[k][e] = a.residual_scale * z[k][e] + ((y[k][e] - st.x) * st.y * G1[k][e] + G0[k][e]);
-        Pack<TS, VEC>::store(h + col.at[k], z[k]);
+            for (int e = 0; e < VEC; ++e) y[k][e] = (y[k][e] - st.x) * st.y * w[e] + o[e];
+          }
       }
+      TS* h = static_cast<TS*>(p.h.ptr) + b * p.h.stride_b + t * p.h.stride_t;
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        if (col.in(k)) {
+          float g[VEC];
+          vector_or<VEC>(p.v.gate, b, f, col.at(k), 1.f, g);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) z[k][e] = p.alpha * z[k][e] + g[e] * y[k][e];
+          Pack<TS, VEC>::store(h + col.at(k), z[k]);
+        }
     }
-    if constexpr (NEXT) {
-      const float2 st = row_stats<VEC, K>(z, col, a.next.kind, a.width, a.next.eps, n_mine, n_lane, sums);
-      if (a.stats && threadIdx.x == 0) reinterpret_cast<float2*>(a.stats)[row] = st;
-      TB* n = static_cast<TB*>(a.n.ptr) + b * a.n.stride_b + t * a.n.stride_t;
+    if (next) {
+      const float2 st = row_stats<VEC, K>(z, col, p.kind, p.eps, n_mine, n_lane, team);
+      if (p.stats && team.warp == 0 && team.lane == 0) p.stats[row] = st;
+      TB* n = static_cast<TB*>(p.n.ptr) + b * p.n.stride_b + t * p.n.stride_t;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!col.in[k]) continue;
-        float o[VEC];
+      for (int k = 0; k < K; ++k)
+        if (col.in(k)) {
+          float o[VEC], m[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = (z[k][e] - st.x) * st.y * A[k][e] + B[k][e];
-        Pack<TB, VEC>::store(n + col.at[k], o);
-      }
+          for (int e = 0; e < VEC; ++e) o[e] = (z[k][e] - st.x) * st.y;
+          if (p.v.weight.ptr) {
+            vector_or<VEC>(p.v.weight, 0, 0, col.at(k), 1.f, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] *= m[e];
+          }
+          if (p.v.bias.ptr) {
+            vector_or<VEC>(p.v.bias, 0, 0, col.at(k), 0.f, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] += m[e];
+          }
+          if (p.v.scale.ptr) {
+            vector_or<VEC>(p.v.scale, b, f, col.at(k), 0.f, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] *= 1.f + m[e];
+          }
+          if (p.v.shift.ptr) {
+            vector_or<VEC>(p.v.shift, b, f, col.at(k), 0.f, m);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] += m[e];
+          }
+          Pack<TB, VEC>::store(n + col.at(k), o);
+        }
     }
   }
 }
 
-template <typename TS, typename TB, bool JOIN, bool NEXT, int VEC, int K>
-int launch(const LvsaBlockNorm& a, cudaStream_t s) {
-  auto kern = block_norm_fwd_kernel<TS, TB, JOIN, NEXT, VEC, K>;
-  const int threads = row_threads(a.width, VEC, K);
+// VEC values an access, K accesses a thread.
+template <typename TS, typename TB, bool JOIN, int VEC, int K>
+int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
+  auto kern = block_norm_fwd_kernel<TS, TB, JOIN, VEC, K>;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.seq;
+  const int vectors = (a.width + VEC - 1) / VEC;
+  const int sms = device_sms();
+  if (sms < 1) return LVSA_ERR_CUDA;
+  // Warps a row: as few as hold it, or one access a thread where the rows do
+  // not fill the device anyway and a row's latency is the time.
+  int warps = (vectors + 32 * K - 1) / (32 * K);
+  if (rows <= 4 * sms) warps = std::min(kWarps<VEC>, (vectors + 31) / 32);
+  int teams = std::max(1, 8 / warps);  // a CTA of 8 warps, or fewer while SMs are left over
+  while (teams > 1 && rows < static_cast<int64_t>(teams) * sms) --teams;
+  const int threads = 32 * warps * teams;
   static std::atomic<int> known[kMaxWarps + 1];
-  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, known);
+  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, 0, known);
   if (ctas < 1) return LVSA_ERR_CUDA;
-  kern<<<static_cast<unsigned>(std::min(rows, ctas)), threads, 0, s>>>(a, rows, a.seq / a.frames);
+  const FwdParams p{a.x, a.y, a.h, a.n, v, FastDiv(a.seq), FastDiv(a.seq / a.frames), static_cast<uint32_t>(rows),
+                    static_cast<uint32_t>(a.frames), a.width, warps, a.next.kind, a.post.kind, a.residual_scale,
+                    a.next.eps, a.post.eps, reinterpret_cast<float2*>(a.stats), reinterpret_cast<float2*>(a.post_stats)};
+  kern<<<static_cast<unsigned>(std::min((rows + teams - 1) / teams, ctas)), threads, 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-template <typename TS, typename TB, bool JOIN, bool NEXT>
+template <typename TS, typename TB, bool JOIN>
 int launch_width(const LvsaBlockNorm& a, cudaStream_t s) {
-  switch (row_shape(a.width, vector_rows<TS, TB>(a))) {
-    case RowShape::kVec1: return launch<TS, TB, JOIN, NEXT, 8, 1>(a, s);
-    case RowShape::kVec2: return launch<TS, TB, JOIN, NEXT, 8, 2>(a, s);
-    case RowShape::kOne8: return launch<TS, TB, JOIN, NEXT, 1, 8>(a, s);
-    default: return launch<TS, TB, JOIN, NEXT, 1, 16>(a, s);
-  }
-}
-
-template <typename TS, typename TB>
-int launch_form(const LvsaBlockNorm& a, cudaStream_t s) {
-  if (!a.y.ptr) return launch_width<TS, TB, false, true>(a, s);
-  return a.n.ptr ? launch_width<TS, TB, true, true>(a, s) : launch_width<TS, TB, true, false>(a, s);
+  constexpr int VEC = kVec<TS>;
+  const Vectors v(a);
+  // Widths, strides or pointers that 16-byte accesses do not fit go value by value.
+  if (a.width % VEC == 0 && rows_vector<TS, VEC>(a.x) && rows_vector<TB, VEC>(a.y) && rows_vector<TS, VEC>(a.h) &&
+      rows_vector<TB, VEC>(a.n) && v.aligned(VEC))
+    return launch<TS, TB, JOIN, VEC, kElems / VEC>(a, v, s);
+  return launch<TS, TB, JOIN, 1, 16>(a, v, s);
 }
 
 }  // namespace
@@ -156,5 +170,9 @@ extern "C" int lvsa_block_norm_fwd(const LvsaBlockNorm* a, void* stream) {
   if (a->y.ptr && !a->h.ptr) return LVSA_ERR_INVALID_ARG;
   if (a->batch == 0 || a->seq == 0) return LVSA_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return by_types(*a, [&](auto ts, auto tb) { return launch_form<decltype(ts), decltype(tb)>(*a, s); });
+  return by_types(*a, [&](auto ts, auto tb) {
+    using TS = decltype(ts);
+    using TB = decltype(tb);
+    return a->y.ptr ? launch_width<TS, TB, true>(*a, s) : launch_width<TS, TB, false>(*a, s);
+  });
 }

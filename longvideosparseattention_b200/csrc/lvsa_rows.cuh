@@ -1,6 +1,6 @@
-// Shared by the block-norm kernels: one CTA works on one row [C] at a time,
-// each thread on fixed columns of it, so that vectors of the channels
-// (modulation, norm weights) and sums over rows stay in its registers.
+// Shared by the block-norm kernels (lvsa_block_norm.cu, lvsa_block_norm_bwd.cu):
+// typed vector accesses, the vectors of the channels, sums over the warps that
+// hold a row, and the host's checks of the arguments.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -28,52 +28,45 @@ __device__ __forceinline__ T from_f(float v) {
   else return v;
 }
 
-// VEC consecutive values of a row in their storage type; 16-byte accesses
-// for VEC = 8 (one for the 2-byte types, two for fp32), plain ones for 1.
+// Storage of VEC values of a type: 1, 8 or 16 bytes (fp32 takes at most 4 values).
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<2> { using type = uint16_t; };
+template <>
+struct Raw<4> { using type = uint32_t; };
+template <>
+struct Raw<8> { using type = uint2; };
+template <>
+struct Raw<16> { using type = uint4; };
+
 template <typename T, int VEC>
-struct Pack;
-template <typename T>
-struct Pack<T, 1> {
-  T v;
-  __device__ __forceinline__ void load(const T* p) { v = __ldg(p); }
-  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f(v); }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[1]) { *p = from_f<T>(f[0]); }
-};
-template <typename T>
-struct Pack<T, 8> {
-  uint4 u;
-  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const uint4*>(p)); }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+struct Pack {
+  using R = typename Raw<static_cast<int>(sizeof(T)) * VEC>::type;
+  R u;
+  __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const R*>(p)); }
+  __device__ __forceinline__ void get(float (&f)[VEC]) const {
     const T* h = reinterpret_cast<const T*>(&u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f(h[i]);
+    for (int i = 0; i < VEC; ++i) f[i] = to_f(h[i]);
   }
-  static __device__ __forceinline__ void store(T* p, const float (&f)[8]) {
-    uint4 o;
+  static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
+    R o;
     T* h = reinterpret_cast<T*>(&o);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = o;
-  }
-};
-template <>
-struct Pack<float, 8> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = __ldg(reinterpret_cast<const float4*>(p));
-    b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&f)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    for (int i = 0; i < VEC; ++i) h[i] = from_f<T>(f[i]);
+    *reinterpret_cast<R*>(p) = o;
   }
 };
 
-// Value i of a vector whose type is known at run time only (modulation and
-// norm parameters: read once a group of rows).
+// A vector of the channels whose type is known at run time (modulation, norm
+// parameters): element strides between sequences and frames, ptr NULL: absent.
+struct Vector {
+  const void* ptr;
+  int64_t stride_b, stride_f;
+  int32_t dtype;
+};
+
 __device__ __forceinline__ float any_load(const void* p, int32_t dtype, int64_t i) {
   if (dtype == LVSA_DTYPE_F32) return __ldg(static_cast<const float*>(p) + i);
   if (dtype == LVSA_DTYPE_BF16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
@@ -84,88 +77,121 @@ __device__ __forceinline__ void any_store(void* p, int32_t dtype, int64_t i, flo
   else if (dtype == LVSA_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
-// VEC consecutive ones from i, or `otherwise` where there is no vector.
+// VEC consecutive values from element i (a multiple of VEC; the host has
+// checked the alignment where VEC > 1).
 template <int VEC>
-__device__ __forceinline__ void any_load(const void* p, int32_t dtype, int64_t i, float otherwise, float (&f)[VEC]) {
-  if (p == nullptr) {
+__device__ __forceinline__ void any_load(const void* p, int32_t dtype, int64_t i, float (&f)[VEC]) {
+  if (dtype == LVSA_DTYPE_F32) {
+    constexpr int E = VEC > 4 ? 4 : VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = otherwise;
-    return;
-  }
-  if constexpr (VEC == 8) {
-    const int64_t at = reinterpret_cast<int64_t>(p) + i * (dtype == LVSA_DTYPE_F32 ? 4 : 2);
-    if ((at & 15) == 0) {
-      if (dtype == LVSA_DTYPE_F32) {
-        Pack<float, 8> q;
-        q.load(static_cast<const float*>(p) + i);
-        q.get(f);
-      } else if (dtype == LVSA_DTYPE_BF16) {
-        Pack<__nv_bfloat16, 8> q;
-        q.load(static_cast<const __nv_bfloat16*>(p) + i);
-        q.get(f);
-      } else {
-        Pack<__half, 8> q;
-        q.load(static_cast<const __half*>(p) + i);
-        q.get(f);
-      }
-      return;
+    for (int j = 0; j < VEC / E; ++j) {
+      Pack<float, E> q;
+      float g[E];
+      q.load(static_cast<const float*>(p) + i + j * E);
+      q.get(g);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[j * E + e] = g[e];
+    }
+  } else {
+    Pack<__half, VEC> q;  // the bits of either 16-bit type
+    q.load(static_cast<const __half*>(p) + i);
+    if (dtype == LVSA_DTYPE_F16) {
+      q.get(f);
+    } else {
+      const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(&q.u);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = __bfloat162float(h[e]);
     }
   }
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) f[e] = any_load(p, dtype, i + e);
 }
+template <int VEC>
+__device__ __forceinline__ void vector_or(const Vector& v, int64_t b, int64_t f, int c, float otherwise, float (&o)[VEC]) {
+  if (v.ptr) {
+    any_load<VEC>(v.ptr, v.dtype, b * v.stride_b + f * v.stride_f + c, o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) o[e] = otherwise;
+  }
+}
+
+// n / d by a multiplication, for n below 2^31: with 2^s >= d and
+// m = floor(2^(31 + s) / d) + 1, n m / 2^(31 + s) is at least n / d and off by
+// less than 2^-s <= 1 / d, which passes no whole number.
+struct FastDiv {
+  uint32_t d, m, s;
+  __host__ explicit FastDiv(uint32_t divisor = 1) : d(divisor), m(0), s(0) {
+    while ((1ull << s) < d) ++s;
+    if (s) m = static_cast<uint32_t>(((1ull << 31) * (1ull << s)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return s ? __umulhi(n << 1, m) >> s : n; }
+};
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Two sums at once: after the first exchange the lower lanes carry a, the
+// upper ones b, so that the pair costs six exchanges rather than ten.
+__device__ __forceinline__ float2 warp_sum2(float a, float b) {
+  const bool up = threadIdx.x & 16;
+  float mine = up ? b : a;
+  mine += __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  const float other = __shfl_xor_sync(0xffffffffu, mine, 16);
+  return up ? make_float2(other, mine) : make_float2(mine, other);
+}
 
 constexpr int kMaxWarps = 32;  // of a CTA
 
-// Sums over the CTA.  One barrier each: the slots alternate, and a thread
-// that writes a slot again has passed the barrier of the call between, which
-// every reader of that slot has reached after reading it.
-struct RowSums {
-  float2 (*slots)[kMaxWarps];  // [2][kMaxWarps], shared
-  int warps, warp, lane, turn;
+// The warps that hold one row: `count` of them, `slots` [2][count] of their
+// own in shared memory, a hardware barrier of their own.  One barrier a sum:
+// the slots alternate, and a thread that writes a slot again has passed the
+// barrier of the sum between, which every reader of the slot has reached
+// after reading it.
+struct Team {
+  float2* slots;
+  int count, warp, lane, barrier, turn;
 
-  __device__ __forceinline__ RowSums(float2 (*s)[kMaxWarps])
-      : slots(s), warps(blockDim.x >> 5), warp(threadIdx.x >> 5), lane(threadIdx.x & 31), turn(0) {}
-
+  __device__ __forceinline__ Team(float2* all, int warps_a_team)
+      : count(warps_a_team), lane(threadIdx.x & 31), turn(0) {
+    const int w = threadIdx.x >> 5, team = w / warps_a_team;
+    warp = w - team * warps_a_team;
+    slots = all + 2 * team * warps_a_team;
+    barrier = team + 1;
+  }
+  // Lane l gets warp l's pair (zeros past the team); alone: every lane its own.
   __device__ __forceinline__ float2 gather(float2 mine) {
-    float2* s = slots[turn];
+    float2* s = slots + turn * count;
     turn ^= 1;
     if (lane == 0) s[warp] = mine;
-    __syncthreads();
-    return lane < warps ? s[lane] : make_float2(0.f, 0.f);
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
+    return lane < count ? s[lane] : make_float2(0.f, 0.f);
   }
   __device__ __forceinline__ float2 sum2(float a, float b) {
-    const float2 g = gather(make_float2(warp_sum(a), warp_sum(b)));
-    return make_float2(warp_sum(g.x), warp_sum(g.y));
+    float2 v = warp_sum2(a, b);
+    if (count > 1) {
+      v = gather(v);
+      v = warp_sum2(v.x, v.y);
+    }
+    return v;
   }
 };
 
-// Columns of one thread: VEC at (t + k T) VEC for k < K.
+// Columns of one thread: VEC at (t + k T) VEC for k < K, T the team's threads.
 template <int VEC, int K>
 struct Columns {
-  int at[K];
-  bool in[K];
-  __device__ __forceinline__ explicit Columns(int width) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      at[k] = (threadIdx.x + k * blockDim.x) * VEC;
-      in[k] = at[k] < width;
-    }
-  }
+  int first, step, width;
+  __device__ __forceinline__ Columns(const Team& t, int w)
+      : first((t.warp * 32 + t.lane) * VEC), step(t.count * 32 * VEC), width(w) {}
+  __device__ __forceinline__ int at(int k) const { return first + k * step; }
+  __device__ __forceinline__ bool in(int k) const { return first + k * step < width; }
   // Values of the row that warp w holds.
-  static __device__ __forceinline__ float of_warp(int w, int width) {
+  __device__ __forceinline__ float of_warp(int w) const {
     int n = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int first = (w * 32 + k * static_cast<int>(blockDim.x)) * VEC;
-      n += max(0, min(32 * VEC, width - first));
-    }
+    for (int k = 0; k < K; ++k) n += max(0, min(32 * VEC, width - (w * 32 * VEC + k * step)));
     return static_cast<float>(n);
   }
 };
@@ -173,82 +199,113 @@ struct Columns {
 // Mean (0 for the RMS norm) and 1 / sqrt(variance + eps) of a row whose
 // columns outside it are zero.  The layer norm's sums are joined from each
 // warp's own mean and squares about it, so that a row's offset does not
-// cancel in the variance, with one barrier.
+// cancel in the variance, with one barrier.  n_mine, n_lane: values that this
+// warp and warp `lane` hold.
 template <int VEC, int K>
-__device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Columns<VEC, K>& col, int kind, int width,
-                                            float eps, float n_mine, float n_lane, RowSums& sums) {
-  const float inv = 1.f / static_cast<float>(width);
+__device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Columns<VEC, K>& col, int kind, float eps,
+                                            float n_mine, float n_lane, Team& team) {
+  const float inv = 1.f / static_cast<float>(col.width);
   if (kind == LVSA_BLOCK_NORM_RMS) {
     float q = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
+      if (col.in(k)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) q += z[k][e] * z[k][e];
-    const float2 g = sums.gather(make_float2(warp_sum(q), 0.f));
-    return make_float2(0.f, rsqrtf(warp_sum(g.x) * inv + eps));
+        for (int e = 0; e < VEC; ++e) q += z[k][e] * z[k][e];
+      }
+    q = warp_sum(q);
+    if (team.count > 1) q = warp_sum(team.gather(make_float2(q, 0.f)).x);
+    return make_float2(0.f, rsqrtf(q * inv + eps));
   }
   float s = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
+    if (col.in(k)) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) s += z[k][e];
+      for (int e = 0; e < VEC; ++e) s += z[k][e];
+    }
   s = warp_sum(s);
   const float mw = s / fmaxf(n_mine, 1.f);
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
+    if (col.in(k)) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float d = col.in[k] ? z[k][e] - mw : 0.f;
-      q += d * d;
+      for (int e = 0; e < VEC; ++e) {
+        const float d = z[k][e] - mw;
+        q += d * d;
+      }
     }
-  const float2 g = sums.gather(make_float2(s, warp_sum(q)));
+  q = warp_sum(q);
+  if (team.count == 1) return make_float2(mw, rsqrtf(q * inv + eps));
+  const float2 g = team.gather(make_float2(s, q));
   const float mean = warp_sum(g.x) * inv;
   const float d = n_lane > 0.f ? g.x / n_lane - mean : 0.f;
-  const float m2 = warp_sum(g.y + n_lane * d * d);
-  return make_float2(mean, rsqrtf(m2 * inv + eps));
+  return make_float2(mean, rsqrtf(warp_sum(g.y + n_lane * d * d) * inv + eps));
 }
 
-// Rows [first, last) of CTA i of n.
+// Rows [first_row(i), first_row(i + 1)) are CTA i's of n; row_owner is its inverse.
 __host__ __device__ __forceinline__ int64_t first_row(int64_t rows, int64_t i, int64_t n) { return rows * i / n; }
+__host__ __device__ __forceinline__ int64_t row_owner(int64_t rows, int64_t row, int64_t n) {
+  return ((row + 1) * n - 1) / rows;
+}
 
 // ------------------------------------------------------------------- host
-// How a row is laid over threads: VEC values a vector, K vectors a thread, at
-// most kMaxWarps warps.  Wide rows take more vectors a thread; widths or
-// strides that 16-byte vectors of 8 values do not fit go value by value.
-enum class RowShape { kVec1, kVec2, kOne8, kOne16 };
+// Values of a vector access to a row: 16 bytes of the stream's type.
+template <typename TS>
+constexpr int kVec = 16 / static_cast<int>(sizeof(TS));
 
-inline int row_threads(int width, int vec, int k) {
-  const int vectors = (width + vec - 1) / vec;
-  return ((vectors + k - 1) / k + 31) / 32 * 32;
-}
-inline RowShape row_shape(int width, bool vectors) {
-  const bool wide = width > 32 * kMaxWarps * 8;
-  return vectors ? (wide ? RowShape::kVec2 : RowShape::kVec1) : (wide ? RowShape::kOne16 : RowShape::kOne8);
-}
-
-template <typename T>
+template <typename T, int VEC>
 inline bool rows_vector(const LvsaRows& r) {
-  constexpr int per = 16 / sizeof(T);
-  return r.ptr == nullptr || ((reinterpret_cast<uintptr_t>(r.ptr) & 15) == 0 && r.stride_b % per == 0 && r.stride_t % per == 0);
+  return r.ptr == nullptr ||
+         ((reinterpret_cast<uintptr_t>(r.ptr) % (sizeof(T) * VEC)) == 0 && r.stride_b % VEC == 0 && r.stride_t % VEC == 0);
 }
-template <typename TS, typename TB>
-inline bool vector_rows(const LvsaBlockNorm& a) {
-  return a.width % 8 == 0 && rows_vector<TS>(a.x) && rows_vector<TB>(a.y) && rows_vector<TS>(a.h) && rows_vector<TB>(a.n);
+inline bool vector_vector(const Vector& v, int vec) {
+  return v.ptr == nullptr || (reinterpret_cast<uintptr_t>(v.ptr) % (v.dtype == LVSA_DTYPE_F32 ? 16 : 2 * vec) == 0 &&
+                              v.stride_b % vec == 0 && v.stride_f % vec == 0);
 }
 
+struct Vectors {
+  Vector gate, scale, shift, weight, bias, post_weight, post_bias;
+  explicit Vectors(const LvsaBlockNorm& a)
+      : gate{a.gate.ptr, a.gate.stride_b, a.gate.stride_f, a.gate.dtype},
+        scale{a.scale.ptr, a.scale.stride_b, a.scale.stride_f, a.scale.dtype},
+        shift{a.shift.ptr, a.shift.stride_b, a.shift.stride_f, a.shift.dtype},
+        weight{a.next.weight, 0, 0, a.next.weight_dtype},
+        bias{a.next.bias, 0, 0, a.next.bias_dtype},
+        post_weight{a.post.weight, 0, 0, a.post.weight_dtype},
+        post_bias{a.post.bias, 0, 0, a.post.bias_dtype} {}
+  bool aligned(int vec) const {
+    for (const Vector* v : {&gate, &scale, &shift, &weight, &bias, &post_weight, &post_bias})
+      if (!vector_vector(*v, vec)) return false;
+    return true;
+  }
+};
+
+inline int device_sms() {
+  static std::atomic<int> known{0};
+  int n = known.load(std::memory_order_relaxed);
+  if (n == 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+      return 0;
+    known.store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
 // CTAs of `kern` that fit the device at once; `known` keeps the answer for
-// each CTA size (the device is always the same chip).
-inline int64_t resident_ctas(const void* kern, int threads, std::atomic<int> (&known)[kMaxWarps + 1]) {
+// each CTA size (every device of a process is the same chip), whose shared
+// memory goes with it.
+inline int64_t resident_ctas(const void* kern, int threads, int shared, std::atomic<int> (&known)[kMaxWarps + 1]) {
   std::atomic<int>& slot = known[threads / 32];
   int n = slot.load(std::memory_order_relaxed);
   if (n == 0) {
-    int dev = 0, sms = 0, per = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess ||
-        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, 0) != cudaSuccess)
+    if (shared > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess)
       return 0;
-    n = sms * per;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, shared) != cudaSuccess) return 0;
+    n *= device_sms();
     slot.store(n, std::memory_order_relaxed);
   }
   return n;
@@ -271,7 +328,8 @@ inline int check_block_norm(const LvsaBlockNorm& a) {
   if (a.batch < 0 || a.seq < 0 || a.frames < 1 || a.width < 1) return LVSA_ERR_INVALID_ARG;
   if (a.seq % a.frames) return LVSA_ERR_GEOMETRY;
   if (!known_type(a.stream_dtype) || !known_type(a.branch_dtype) || a.width > LVSA_BLOCK_NORM_MAX_WIDTH ||
-      (a.stream_dtype != a.branch_dtype && a.stream_dtype != LVSA_DTYPE_F32))
+      (a.stream_dtype != a.branch_dtype && a.stream_dtype != LVSA_DTYPE_F32) ||
+      static_cast<int64_t>(a.batch) * a.seq > LVSA_BLOCK_NORM_MAX_ROWS)
     return LVSA_ERR_UNSUPPORTED;
   for (const LvsaVectors* v : {&a.gate, &a.scale, &a.shift})
     if (v->ptr && !known_type(v->dtype)) return LVSA_ERR_UNSUPPORTED;
