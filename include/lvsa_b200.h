@@ -315,7 +315,7 @@ int lvsa_copy_segments(const LvsaCopySegment* segs, int32_t n, int32_t row_bytes
  * tokens to each frame; a stride of 0 shares a vector.  fp32 arithmetic, one
  * rounding of each output; n is of h before its rounding. */
 enum { LVSA_BLOCK_NORM_NONE = 0, LVSA_BLOCK_NORM_LAYER = 1, LVSA_BLOCK_NORM_RMS = 2 };
-#define LVSA_BLOCK_NORM_MAX_WIDTH 16384
+#define LVSA_BLOCK_NORM_MAX_WIDTH 8192
 #define LVSA_BLOCK_NORM_MAX_ROWS 2147483000 /* batch * seq */
 typedef struct LvsaRows { /* [batch, seq, width], width contiguous; element strides */
   void* ptr;

@@ -96,7 +96,7 @@ class LvsaQkPrologue(ctypes.Structure):
 
 
 LVSA_BLOCK_NORM_NONE, LVSA_BLOCK_NORM_LAYER, LVSA_BLOCK_NORM_RMS = 0, 1, 2
-LVSA_BLOCK_NORM_MAX_WIDTH = 16384
+LVSA_BLOCK_NORM_MAX_WIDTH = 8192
 
 
 class LvsaRows(ctypes.Structure):

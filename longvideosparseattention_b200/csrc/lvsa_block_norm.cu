@@ -2,11 +2,17 @@
 // residual scale:
 //   h = a x + gate * post(y),   n = next(h) * (1 + scale) + shift.
 //
-// A team of warps holds one row in registers, kElems values a thread at most
-// (one warp up to 1024 channels, so that its sums need no barrier), and walks
-// rows a grid's teams apart.  Modulation and norm weights are read again for
-// every row: they are the same few kilobytes for all rows of a frame and stay
-// in L1, where holding them in registers would halve the rows in flight.
+// With zhat the normalised row, next's weight and the modulation fold to
+// n = zhat A + B, A = w (1 + scale), B = b (1 + scale) + shift, and post's
+// weight and the gate to h = a x + yhat G1 + G0.
+//
+// A CTA takes consecutive rows and keeps the fp32 vectors of the group (the
+// tokens of a frame) that it is in in shared memory; its teams of warps take
+// the group's rows in turn, a row in a team's registers, kElems values a
+// thread at most (one warp up to 1024 channels, whose sums need no barrier).
+// As soon as a row's values are taken from it, a thread's slot of shared
+// memory is filled with its part of the team's next row (cp.async), so that
+// every warp has a row on its way at all times without registers for it.
 // Bound: HBM (x and y read once, h and n written once).
 #include <algorithm>
 #include <atomic>
@@ -17,116 +23,240 @@ namespace lvsa {
 namespace {
 
 constexpr int kElems = 32;
+// Threads of a CTA at most: 80 registers each, 96 where both rows are held at
+// once (a norm of the branch), 128 where the next row waits in registers.
+template <int VEC, int FORM>
+constexpr int kThreads = VEC == 1 ? 512 : FORM == 2 ? 640 : 768;
+
+__host__ __device__ inline int shared_pitch(int width) { return (width + 7) & ~7; }
 
 struct FwdParams {
   LvsaRows x, y, h, n;
   Vectors v;
   FastDiv by_seq, by_group;  // row -> sequence; row -> group (frame of a sequence)
   uint32_t rows, frames;
-  int32_t width, warps, kind, post_kind;
+  int32_t width, warps, vectors_held, kind, post_kind;
   float alpha, eps, post_eps;
   float2 *stats, *post_stats;
 };
 
-// Warps of a CTA at most: kElems values a thread hold the widest row in 16.
-template <int VEC>
-constexpr int kWarps = VEC == 1 ? kMaxWarps : 16;
+// Vectors of channels in shared memory, `pitch` floats each.  Of 8 values the
+// first and last four lie half a vector apart, so that the lanes of a warp
+// touch consecutive 16 bytes.
+enum { kA = 0, kB = 1, kG1 = 2, kG0 = 3 };
 
-template <typename TS, typename TB, bool JOIN, int VEC, int K>
-__global__ void __launch_bounds__(32 * kWarps<VEC>) block_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
+template <int VEC>
+struct SharedVector {
+  static constexpr int kQuads = VEC == 1 ? 1 : VEC / 4;
+  using Q = typename std::conditional<VEC == 1, float, float4>::type;
+  Q* quad[kQuads];  // this thread's first
+
+  __device__ __forceinline__ SharedVector(float* all, int pitch, int which, int column) {
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+      quad[j] = reinterpret_cast<Q*>(all + which * pitch + j * (pitch / kQuads)) + column / VEC;
+  }
+  // At `vectors` (a constant) from the first.
+  __device__ __forceinline__ void get(int vectors, float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      f[0] = quad[0][vectors];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) {
+        const float4 q = quad[j][vectors];
+        f[4 * j] = q.x; f[4 * j + 1] = q.y; f[4 * j + 2] = q.z; f[4 * j + 3] = q.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(const float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      quad[0][0] = f[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) quad[j][0] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+    }
+  }
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+
+// FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
+template <typename TS, typename TB, int FORM, int VEC, int K>
+__global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
   __shared__ float2 slots[2 * kMaxWarps];
+  extern __shared__ float4 shared_vectors[];
+  float* const held = reinterpret_cast<float*>(shared_vectors);
+  const int pitch = shared_pitch(p.width);
+  constexpr bool RING = VEC > 1, JOIN = FORM > 0, POST = FORM == 2;
+  using RX = typename Pack<TS, VEC>::R;
+  using RY = typename Pack<TB, VEC>::R;
+  const int slot = (threadIdx.x >> 5) * K * 32 + (threadIdx.x & 31);
+  RX* const x_slot = reinterpret_cast<RX*>(held + p.vectors_held * pitch) + slot;
+  RY* const y_slot = reinterpret_cast<RY*>(x_slot - slot + K * blockDim.x) + slot;
   Team team(slots, p.warps);
   const Columns<VEC, K> col(team, p.width);
-  const float n_mine = col.of_warp(team.warp), n_lane = team.lane < team.count ? col.of_warp(team.lane) : 0.f;
-  const uint32_t teams = blockDim.x / (32 * p.warps);
-  const bool next = !JOIN || p.n.ptr;
+  __shared__ float counts[kMaxWarps];
+  const Held share(counts, col, team);
+  const SharedVector<VEC> vkA(held, pitch, kA, col.first), vkB(held, pitch, kB, col.first);
+  const SharedVector<VEC> vkG1(held, pitch, JOIN ? kG1 : 0, col.first), vkG0(held, pitch, POST ? kG0 : 0, col.first);
+  const uint32_t teams = blockDim.x / (32 * p.warps), mine = team.barrier - 1;
+  const bool next = !JOIN || p.n.ptr, g0 = POST && p.v.post_bias.ptr;
+  const uint32_t r1 = static_cast<uint32_t>(first_row(p.rows, blockIdx.x + 1, gridDim.x));
 
-  for (uint32_t row = blockIdx.x * teams + team.barrier - 1; row < p.rows; row += gridDim.x * teams) {
-    const uint32_t b = p.by_seq.div(row);
-    const int64_t t = row - b * p.by_seq.d, f = p.by_group.div(row) - b * p.frames;
-    float z[K][VEC];
-    const TS* x = static_cast<const TS*>(p.x.ptr) + b * p.x.stride_b + t * p.x.stride_t;
+  uint32_t end;
+  for (uint32_t start = static_cast<uint32_t>(first_row(p.rows, blockIdx.x, gridDim.x)); start < r1; start = end) {
+    const uint32_t group = p.by_group.div(start);
+    end = min(r1, (group + 1) * p.by_group.d);
+    const int64_t b = p.by_seq.div(start), f = group - b * p.frames;
+    const int64_t t0 = start + mine - b * p.by_seq.d;  // the team's first token in the sequence
+    __syncthreads();
+    for (int c = threadIdx.x * VEC; c < p.width; c += blockDim.x * VEC) {
+      float w[VEC], o[VEC], m[VEC];
+      if (next) {
+        vector_or<VEC>(p.v.weight, 0, 0, c, 1.f, w);
+        vector_or<VEC>(p.v.bias, 0, 0, c, 0.f, o);
+        vector_or<VEC>(p.v.scale, b, f, c, 0.f, m);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (col.in(k)) {
-        Pack<TS, VEC> q;
-        q.load(x + col.at(k));
-        q.get(z[k]);
+        for (int e = 0; e < VEC; ++e) {
+          w[e] *= 1.f + m[e];
+          o[e] *= 1.f + m[e];
+        }
+        vector_or<VEC>(p.v.shift, b, f, c, 0.f, m);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) o[e] += m[e];
+        SharedVector<VEC>(held, pitch, kA, c).put(w);
+        SharedVector<VEC>(held, pitch, kB, c).put(o);
       }
-    if constexpr (JOIN) {
-      float y[K][VEC];
-      const TB* yp = static_cast<const TB*>(p.y.ptr) + b * p.y.stride_b + t * p.y.stride_t;
+      if constexpr (JOIN) {
+        vector_or<VEC>(p.v.gate, b, f, c, 1.f, m);
+        vector_or<VEC>(p.v.post_weight, 0, 0, c, 1.f, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] *= m[e];
+        SharedVector<VEC>(held, pitch, kG1, c).put(w);
+        if (g0) {
+          vector_or<VEC>(p.v.post_bias, 0, 0, c, 0.f, o);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] *= m[e];
+          SharedVector<VEC>(held, pitch, kG0, c).put(o);
+        }
+      }
+    }
+    __syncthreads();
+
+    // The team's next row: in this thread's slots, or in registers where a
+    // value is too small for an asynchronous copy.
+    Pack<TS, VEC> xs[RING ? 1 : K];
+    Pack<TB, VEC> ys[RING || !JOIN ? 1 : K];
+    const TS* x = static_cast<const TS*>(p.x.ptr) + b * p.x.stride_b + t0 * p.x.stride_t + col.first;
+    const TB* y = JOIN ? static_cast<const TB*>(p.y.ptr) + b * p.y.stride_b + t0 * p.y.stride_t + col.first : nullptr;
+    TS* h = JOIN ? static_cast<TS*>(p.h.ptr) + b * p.h.stride_b + t0 * p.h.stride_t + col.first : nullptr;
+    TB* n = static_cast<TB*>(p.n.ptr) + b * p.n.stride_b + t0 * p.n.stride_t + col.first;
+    auto fetch = [&]() {
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (col.in(k)) {
-          Pack<TB, VEC> q;
-          q.load(yp + col.at(k));
-          q.get(y[k]);
+          if constexpr (RING) {
+            copy_async<sizeof(TS) * VEC>(x_slot + 32 * k, x + k * col.kStep);
+            if constexpr (JOIN) copy_async<sizeof(TB) * VEC>(y_slot + 32 * k, y + k * col.kStep);
+          } else {
+            xs[k].load(x + k * col.kStep);
+            if constexpr (JOIN) ys[k].load(y + k * col.kStep);
+          }
         }
-      if (p.post_kind != LVSA_BLOCK_NORM_NONE) {
-        const float2 st = row_stats<VEC, K>(y, col, p.post_kind, p.post_eps, n_mine, n_lane, team);
-        if (p.post_stats && team.warp == 0 && team.lane == 0) p.post_stats[row] = st;
+      x += teams * p.x.stride_t;
+      if constexpr (JOIN) y += teams * p.y.stride_t;
+    };
+    auto take_x = [&](int k, float(&f)[VEC]) {
+      if constexpr (RING) {
+        Pack<TS, VEC> q;
+        q.u = x_slot[32 * k];
+        q.get(f);
+      } else {
+        xs[k].get(f);
+      }
+    };
+    auto take_y = [&](int k, float(&f)[VEC]) {
+      if constexpr (RING) {
+        Pack<TB, VEC> q;
+        q.u = y_slot[32 * k];
+        q.get(f);
+      } else {
+        ys[k].get(f);
+      }
+    };
+    if (start + mine < end) fetch();
+    for (uint32_t row = start + mine; row < end; row += teams) {
+      float z[K][VEC];
+      if constexpr (RING) asm volatile("cp.async.wait_all;" ::: "memory");
+      if constexpr (JOIN) {
+        float2 st = make_float2(0.f, 1.f);
+        if constexpr (POST) {
+          float all[K][VEC];
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (col.in(k)) take_y(k, all[k]);
+          st = row_stats<VEC, K>(all, col, p.post_kind, p.post_eps, share, team);
+          if (p.post_stats && team.warp == 0 && team.lane == 0) p.post_stats[row] = st;
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (col.in(k)) {
-            float w[VEC], o[VEC];
-            vector_or<VEC>(p.v.post_weight, 0, 0, col.at(k), 1.f, w);
-            vector_or<VEC>(p.v.post_bias, 0, 0, col.at(k), 0.f, o);
+            float branch[VEC], g[VEC];
+            take_x(k, z[k]);
+            take_y(k, branch);
+            if constexpr (POST) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) y[k][e] = (y[k][e] - st.x) * st.y * w[e] + o[e];
+              for (int e = 0; e < VEC; ++e) branch[e] = (branch[e] - st.x) * st.y;
+            }
+            vkG1.get(32 * k, g);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) z[k][e] = p.alpha * z[k][e] + branch[e] * g[e];
+            if (g0) {
+              vkG0.get(32 * k, g);
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) z[k][e] += g[e];
+            }
           }
+      } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (col.in(k)) take_x(k, z[k]);
       }
-      TS* h = static_cast<TS*>(p.h.ptr) + b * p.h.stride_b + t * p.h.stride_t;
+      if (row + teams < end) fetch();
+      if constexpr (JOIN) {
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (col.in(k)) {
-          float g[VEC];
-          vector_or<VEC>(p.v.gate, b, f, col.at(k), 1.f, g);
+        for (int k = 0; k < K; ++k)
+          if (col.in(k)) Pack<TS, VEC>::store(h + k * col.kStep, z[k]);
+        h += teams * p.h.stride_t;
+      }
+      if (next) {
+        const float2 st = row_stats<VEC, K>(z, col, p.kind, p.eps, share, team);
+        if (p.stats && team.warp == 0 && team.lane == 0) p.stats[row] = st;
+        const float mr = st.x * st.y;
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) z[k][e] = p.alpha * z[k][e] + g[e] * y[k][e];
-          Pack<TS, VEC>::store(h + col.at(k), z[k]);
-        }
-    }
-    if (next) {
-      const float2 st = row_stats<VEC, K>(z, col, p.kind, p.eps, n_mine, n_lane, team);
-      if (p.stats && team.warp == 0 && team.lane == 0) p.stats[row] = st;
-      TB* n = static_cast<TB*>(p.n.ptr) + b * p.n.stride_b + t * p.n.stride_t;
+        for (int k = 0; k < K; ++k)
+          if (col.in(k)) {
+            float A[VEC], B[VEC];
+            vkA.get(32 * k, A);
+            vkB.get(32 * k, B);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (col.in(k)) {
-          float o[VEC], m[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) o[e] = (z[k][e] - st.x) * st.y;
-          if (p.v.weight.ptr) {
-            vector_or<VEC>(p.v.weight, 0, 0, col.at(k), 1.f, m);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o[e] *= m[e];
+            for (int e = 0; e < VEC; ++e) A[e] = (z[k][e] * st.y - mr) * A[e] + B[e];
+            Pack<TB, VEC>::store(n + k * col.kStep, A);
           }
-          if (p.v.bias.ptr) {
-            vector_or<VEC>(p.v.bias, 0, 0, col.at(k), 0.f, m);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o[e] += m[e];
-          }
-          if (p.v.scale.ptr) {
-            vector_or<VEC>(p.v.scale, b, f, col.at(k), 0.f, m);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o[e] *= 1.f + m[e];
-          }
-          if (p.v.shift.ptr) {
-            vector_or<VEC>(p.v.shift, b, f, col.at(k), 0.f, m);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) o[e] += m[e];
-          }
-          Pack<TB, VEC>::store(n + col.at(k), o);
-        }
+        n += teams * p.n.stride_t;
+      }
     }
   }
 }
 
 // VEC values an access, K accesses a thread.
-template <typename TS, typename TB, bool JOIN, int VEC, int K>
+template <typename TS, typename TB, int FORM, int VEC, int K>
 int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
-  auto kern = block_norm_fwd_kernel<TS, TB, JOIN, VEC, K>;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.seq;
   const int vectors = (a.width + VEC - 1) / VEC;
   const int sms = device_sms();
@@ -134,29 +264,43 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
   // Warps a row: as few as hold it, or one access a thread where the rows do
   // not fill the device anyway and a row's latency is the time.
   int warps = (vectors + 32 * K - 1) / (32 * K);
-  if (rows <= 4 * sms) warps = std::min(kWarps<VEC>, (vectors + 31) / 32);
-  int teams = std::max(1, 8 / warps);  // a CTA of 8 warps, or fewer while SMs are left over
-  while (teams > 1 && rows < static_cast<int64_t>(teams) * sms) --teams;
+  if (rows <= 4 * sms) warps = std::max(warps, std::min(16, (vectors + 31) / 32));
+  // Teams a CTA: one CTA fills an SM, its vectors held once; fewer while SMs
+  // are left over or a group has few rows to share its vectors.
+  int teams = std::max(1, std::min(kThreads<VEC, FORM> / (32 * warps), warps == 1 ? 32 : 15));
+  while (teams > 1 && (rows < static_cast<int64_t>(teams) * sms || a.seq / a.frames < 4 * teams)) --teams;
   const int threads = 32 * warps * teams;
-  static std::atomic<int> known[kMaxWarps + 1];
-  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, 0, known);
+  constexpr bool JOIN = FORM > 0;
+  const int vectors_held = !JOIN ? 2 : a.post.bias ? 4 : 3;
+  const int shared = vectors_held * shared_pitch(a.width) * static_cast<int>(sizeof(float)) +
+                     (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + (JOIN ? sizeof(TB) : 0)) : 0);
+  auto kern = block_norm_fwd_kernel<TS, TB, FORM, VEC, K>;
+  static std::atomic<uint64_t> last{0};
+  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
   const FwdParams p{a.x, a.y, a.h, a.n, v, FastDiv(a.seq), FastDiv(a.seq / a.frames), static_cast<uint32_t>(rows),
-                    static_cast<uint32_t>(a.frames), a.width, warps, a.next.kind, a.post.kind, a.residual_scale,
+                    static_cast<uint32_t>(a.frames), a.width, warps, vectors_held, a.next.kind, a.post.kind, a.residual_scale,
                     a.next.eps, a.post.eps, reinterpret_cast<float2*>(a.stats), reinterpret_cast<float2*>(a.post_stats)};
-  kern<<<static_cast<unsigned>(std::min((rows + teams - 1) / teams, ctas)), threads, 0, s>>>(p);
+  kern<<<static_cast<unsigned>(std::min((rows + teams - 1) / teams, ctas)), threads, shared, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-template <typename TS, typename TB, bool JOIN>
+template <typename TS, typename TB, int FORM>
 int launch_width(const LvsaBlockNorm& a, cudaStream_t s) {
   constexpr int VEC = kVec<TS>;
   const Vectors v(a);
   // Widths, strides or pointers that 16-byte accesses do not fit go value by value.
   if (a.width % VEC == 0 && rows_vector<TS, VEC>(a.x) && rows_vector<TB, VEC>(a.y) && rows_vector<TS, VEC>(a.h) &&
-      rows_vector<TB, VEC>(a.n) && v.aligned(VEC))
-    return launch<TS, TB, JOIN, VEC, kElems / VEC>(a, v, s);
-  return launch<TS, TB, JOIN, 1, 16>(a, v, s);
+      rows_vector<TB, VEC>(a.n) && v.aligned(VEC)) {
+    // The fewest warps of kElems values a thread, then the fewest values.
+    const int vectors = a.width / VEC, warps = (vectors * VEC + 32 * kElems - 1) / (32 * kElems);
+    const int k = (vectors + 32 * warps - 1) / (32 * warps);
+    constexpr int kMost = kElems / VEC;
+    return k > kMost * 3 / 4 ? launch<TS, TB, FORM, VEC, kMost>(a, v, s)
+           : k > kMost / 2   ? launch<TS, TB, FORM, VEC, kMost * 3 / 4>(a, v, s)
+                             : launch<TS, TB, FORM, VEC, kMost / 2>(a, v, s);
+  }
+  return launch<TS, TB, FORM, 1, 16>(a, v, s);
 }
 
 }  // namespace
@@ -173,6 +317,7 @@ extern "C" int lvsa_block_norm_fwd(const LvsaBlockNorm* a, void* stream) {
   return by_types(*a, [&](auto ts, auto tb) {
     using TS = decltype(ts);
     using TB = decltype(tb);
-    return a->y.ptr ? launch_width<TS, TB, true>(*a, s) : launch_width<TS, TB, false>(*a, s);
+    if (!a->y.ptr) return launch_width<TS, TB, 0>(*a, s);
+    return a->post.kind == LVSA_BLOCK_NORM_NONE ? launch_width<TS, TB, 1>(*a, s) : launch_width<TS, TB, 2>(*a, s);
   });
 }

@@ -385,10 +385,10 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   auto kern = block_norm_bwd_kernel<TS, TB, FORM, VEC, K, THREADS>;
   const int vectors = (g.f.width + VEC - 1) / VEC;
   const int threads = ((vectors + K - 1) / K + 31) / 32 * 32;
-  static std::atomic<int> known[kMaxWarps + 1];
+  static std::atomic<uint64_t> last{0};
   const int64_t rows = static_cast<int64_t>(g.f.batch) * g.f.seq;
   const int shared = (FORM + 1) * threads * VEC * K * static_cast<int>(sizeof(float));
-  const int64_t ctas = std::min<int64_t>(rows, resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, known));
+  const int64_t ctas = std::min<int64_t>(rows, resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last));
   if (ctas < 1) return LVSA_ERR_CUDA;
   if (ctas_only) {
     *ctas_only = ctas;
@@ -414,11 +414,10 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   const int width = g.f.width;
   if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
       !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC))
-    return width <= 16 * 512 ? launch<TS, TB, FORM, 1, 16, 512>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 1024>(g, v, ctas, s);
+    return launch<TS, TB, FORM, 1, 16, 512>(g, v, ctas, s);
   if (width <= 8 * 384) return launch<TS, TB, FORM, VEC, 8 / VEC, 384>(g, v, ctas, s);
   if (width <= 8 * 672) return launch<TS, TB, FORM, VEC, 8 / VEC, 672>(g, v, ctas, s);
-  if (width <= 16 * 512) return launch<TS, TB, FORM, VEC, 16 / VEC, 512>(g, v, ctas, s);
-  return launch<TS, TB, FORM, VEC, 16 / VEC, 1024>(g, v, ctas, s);
+  return launch<TS, TB, FORM, VEC, 16 / VEC, 512>(g, v, ctas, s);
 }
 
 template <typename TS, typename TB>

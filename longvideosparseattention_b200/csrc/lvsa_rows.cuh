@@ -52,9 +52,19 @@ struct Pack {
   }
   static __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
     R o;
-    T* h = reinterpret_cast<T*>(&o);
+    if constexpr (sizeof(T) == 2 && VEC > 1) {  // pairs: one conversion each
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) h[i] = from_f<T>(f[i]);
+      for (int i = 0; i < VEC / 2; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value)
+          reinterpret_cast<__nv_bfloat162*>(&o)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+        else
+          reinterpret_cast<__half2*>(&o)[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      }
+    } else {
+      T* h = reinterpret_cast<T*>(&o);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[i] = from_f<T>(f[i]);
+    }
     *reinterpret_cast<R*>(p) = o;
   }
 };
@@ -161,50 +171,69 @@ struct Team {
     slots = all + 2 * team * warps_a_team;
     barrier = team + 1;
   }
-  // Lane l gets warp l's pair (zeros past the team); alone: every lane its own.
-  __device__ __forceinline__ float2 gather(float2 mine) {
+  // Every warp's pair, after the barrier.
+  __device__ __forceinline__ const float2* exchange(float2 mine) {
     float2* s = slots + turn * count;
     turn ^= 1;
     if (lane == 0) s[warp] = mine;
-    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
-    return lane < count ? s[lane] : make_float2(0.f, 0.f);
+    if (count * 32 == blockDim.x) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
+    return s;
   }
+  // Few warps are added one after another by every thread, many by exchanges.
   __device__ __forceinline__ float2 sum2(float a, float b) {
     float2 v = warp_sum2(a, b);
-    if (count > 1) {
-      v = gather(v);
-      v = warp_sum2(v.x, v.y);
+    if (count == 1) return v;
+    const float2* s = exchange(v);
+    if (count <= kFew) {
+      v = s[0];
+      for (int w = 1; w < count; ++w) {
+        v.x += s[w].x;
+        v.y += s[w].y;
+      }
+      return v;
     }
-    return v;
+    v = lane < count ? s[lane] : make_float2(0.f, 0.f);
+    return warp_sum2(v.x, v.y);
   }
+  static constexpr int kFew = 6;
 };
 
-// Columns of one thread: VEC at (t + k T) VEC for k < K, T the team's threads.
+// Columns of one thread: a warp holds K x 32 vectors of VEC side by side, the
+// lane's k-th at first + k * kStep (a constant apart: an address for all).
 template <int VEC, int K>
 struct Columns {
-  int first, step, width;
-  __device__ __forceinline__ Columns(const Team& t, int w)
-      : first((t.warp * 32 + t.lane) * VEC), step(t.count * 32 * VEC), width(w) {}
-  __device__ __forceinline__ int at(int k) const { return first + k * step; }
-  __device__ __forceinline__ bool in(int k) const { return first + k * step < width; }
+  static constexpr int kStep = 32 * VEC;
+  int first, width;
+  __device__ __forceinline__ Columns(const Team& t, int w) : first((t.warp * K * 32 + t.lane) * VEC), width(w) {}
+  __device__ __forceinline__ int at(int k) const { return first + k * kStep; }
+  __device__ __forceinline__ bool in(int k) const { return first + k * kStep < width; }
   // Values of the row that warp w holds.
   __device__ __forceinline__ float of_warp(int w) const {
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k) n += max(0, min(32 * VEC, width - (w * 32 * VEC + k * step)));
-    return static_cast<float>(n);
+    return static_cast<float>(max(0, min(K * kStep, width - w * K * kStep)));
   }
 };
 
-// Mean (0 for the RMS norm) and 1 / sqrt(variance + eps) of a row whose
-// columns outside it are zero.  The layer norm's sums are joined from each
-// warp's own mean and squares about it, so that a row's offset does not
-// cancel in the variance, with one barrier.  n_mine, n_lane: values that this
-// warp and warp `lane` hold.
+// How many of a row's values each warp of a team holds (shared memory, filled
+// by every thread of the CTA with the same numbers) and this warp's reciprocal.
+struct Held {
+  const float* counts;
+  float inv_mine, inv_row;
+  template <int VEC, int K>
+  __device__ __forceinline__ Held(float* space, const Columns<VEC, K>& col, const Team& team) : counts(space) {
+    if (team.lane < team.count) space[team.lane] = col.of_warp(team.lane);
+    __syncthreads();
+    inv_mine = 1.f / fmaxf(space[team.warp], 1.f);
+    inv_row = 1.f / static_cast<float>(col.width);
+  }
+};
+
+// Mean (0 for the RMS norm) and 1 / sqrt(variance + eps) of a row.  The layer
+// norm's sums are joined from each warp's own mean and squares about it, so
+// that a row's offset does not cancel in the variance, with one barrier.
 template <int VEC, int K>
 __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Columns<VEC, K>& col, int kind, float eps,
-                                            float n_mine, float n_lane, Team& team) {
-  const float inv = 1.f / static_cast<float>(col.width);
+                                            const Held& held, Team& team) {
   if (kind == LVSA_BLOCK_NORM_RMS) {
     float q = 0.f;
 #pragma unroll
@@ -214,34 +243,56 @@ __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Colu
         for (int e = 0; e < VEC; ++e) q += z[k][e] * z[k][e];
       }
     q = warp_sum(q);
-    if (team.count > 1) q = warp_sum(team.gather(make_float2(q, 0.f)).x);
-    return make_float2(0.f, rsqrtf(q * inv + eps));
+    if (team.count > 1) {
+      const float2* g = team.exchange(make_float2(q, 0.f));
+      if (team.count <= Team::kFew) {
+        q = g[0].x;
+        for (int w = 1; w < team.count; ++w) q += g[w].x;
+      } else {
+        q = warp_sum(team.lane < team.count ? g[team.lane].x : 0.f);
+      }
+    }
+    return make_float2(0.f, rsqrtf(q * held.inv_row + eps));
   }
-  float s = 0.f;
+  float mean = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
     if (col.in(k)) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s += z[k][e];
+      for (int e = 0; e < VEC; ++e) mean += z[k][e];
     }
-  s = warp_sum(s);
-  const float mw = s / fmaxf(n_mine, 1.f);
+  mean = warp_sum(mean) * held.inv_mine;
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k)
     if (col.in(k)) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float d = z[k][e] - mw;
+        const float d = z[k][e] - mean;
         q += d * d;
       }
     }
   q = warp_sum(q);
-  if (team.count == 1) return make_float2(mw, rsqrtf(q * inv + eps));
-  const float2 g = team.gather(make_float2(s, q));
-  const float mean = warp_sum(g.x) * inv;
-  const float d = n_lane > 0.f ? g.x / n_lane - mean : 0.f;
-  return make_float2(mean, rsqrtf(warp_sum(g.y + n_lane * d * d) * inv + eps));
+  if (team.count > 1) {
+    const float2* g = team.exchange(make_float2(mean, q));
+    if (team.count <= Team::kFew) {
+      mean = 0.f;
+      for (int w = 0; w < team.count; ++w) mean += held.counts[w] * g[w].x;
+      mean *= held.inv_row;
+      q = 0.f;
+      for (int w = 0; w < team.count; ++w) {
+        const float d = g[w].x - mean;
+        q += g[w].y + held.counts[w] * d * d;
+      }
+    } else {
+      const float2 m = team.lane < team.count ? g[team.lane] : make_float2(0.f, 0.f);
+      const float n = team.lane < team.count ? held.counts[team.lane] : 0.f;
+      mean = warp_sum(n * m.x) * held.inv_row;
+      const float d = m.x - mean;
+      q = warp_sum(m.y + n * d * d);
+    }
+  }
+  return make_float2(mean, rsqrtf(q * held.inv_row + eps));
 }
 
 // Rows [first_row(i), first_row(i + 1)) are CTA i's of n; row_owner is its inverse.
@@ -294,20 +345,20 @@ inline int device_sms() {
   }
   return n;
 }
-// CTAs of `kern` that fit the device at once; `known` keeps the answer for
-// each CTA size (every device of a process is the same chip), whose shared
-// memory goes with it.
-inline int64_t resident_ctas(const void* kern, int threads, int shared, std::atomic<int> (&known)[kMaxWarps + 1]) {
-  std::atomic<int>& slot = known[threads / 32];
-  int n = slot.load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (shared > 48 * 1024 &&
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess)
-      return 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, shared) != cudaSuccess) return 0;
-    n *= device_sms();
-    slot.store(n, std::memory_order_relaxed);
-  }
+// CTAs of `kern` that fit the device at once.  `last` keeps the answer for the
+// last shape asked for (every device of a process is the same chip; the
+// permission for more than 48 KB of shared memory is each device's own).
+inline int64_t resident_ctas(const void* kern, int threads, int shared, std::atomic<uint64_t>& last) {
+  if (shared > 40 * 1024 &&  // with what a kernel declares itself, 48 KB need no permission
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess)
+    return 0;
+  const uint64_t shape = static_cast<uint64_t>(shared) << 32 | static_cast<uint64_t>(threads) << 16;
+  const uint64_t seen = last.load(std::memory_order_relaxed);
+  if (seen >> 16 == shape >> 16 && (seen & 0xffff)) return seen & 0xffff;
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, shared) != cudaSuccess) return 0;
+  n *= device_sms();
+  last.store(shape | static_cast<uint64_t>(n), std::memory_order_relaxed);
   return n;
 }
 

@@ -92,8 +92,8 @@ def _sizes(t, norm, post, alpha, eps=1e-6):
 
 
 SHAPES = [  # B, S, F, C
-    (1, 1, 1, 8), (1, 3, 3, 1), (2, 77, 1, 2048), (1, 35, 5, 1155), (2, 12, 4, 264), (1, 300, 1, 5120), (1, 9, 3, 8200),
-    (1, 4, 1, 16384), (1, 3, 1, 16383), (2, 5000, 5, 64), (1, 40, 40, 128), (1, 2600, 2, 1536), (3, 7, 7, 9)]
+    (1, 1, 1, 8), (1, 3, 3, 1), (2, 77, 1, 2048), (1, 35, 5, 1155), (2, 12, 4, 264), (1, 300, 1, 5120), (1, 9, 3, 6144),
+    (1, 4, 1, 8192), (1, 3, 1, 8191), (2, 5000, 5, 64), (1, 40, 40, 128), (1, 2600, 2, 1536), (3, 7, 7, 9)]
 TYPES = [(BF, BF, BF), (HF, HF, F32), (F32, BF, F32), (F32, HF, HF), (F32, F32, F32), (BF, BF, F32)]
 FORMS = [  # norm, affine, post, alpha, join
     ("layer", False, None, 1.0, False), ("rms", True, None, 1.0, False), ("layer", True, None, 0.5, True),
@@ -388,7 +388,7 @@ def test_refusals_on_cuda_tensors():
         lambda: norm_modulate(x, scale=torch.zeros(2, 4, 16, device="cuda")),
         lambda: norm_modulate(x, scale=torch.zeros(2, 2, 16, device="cuda"), shift=torch.zeros(2, 3, 16, device="cuda")),
         lambda: norm_modulate(x, scale=torch.zeros(16)), lambda: norm_modulate(x, eps=-1.0),
-        lambda: norm_modulate(torch.zeros(1, 1, 16392, device="cuda")),
+        lambda: norm_modulate(torch.zeros(1, 1, 8193, device="cuda")),
         lambda: gate_residual(x, x[:, :3]), lambda: gate_residual(x, x, post_weight=v),
         lambda: gate_residual(x, x, post_norm="rms", post_bias=v), lambda: gate_residual_norm(x, x, norm=None),
         lambda: gate_residual(x, x, gate=torch.zeros(2, 0, 16, device="cuda")), lambda: gate_residual(x, None)]
