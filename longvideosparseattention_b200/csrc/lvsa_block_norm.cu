@@ -28,7 +28,8 @@ constexpr int kElems = 32;
 template <int VEC, int FORM>
 constexpr int kThreads = VEC == 1 ? 512 : FORM == 2 ? 640 : 768;
 
-__host__ __device__ inline int shared_pitch(int width) { return (width + 7) & ~7; }
+// The vectors held.
+enum { kA = 0, kB = 1, kG1 = 2, kG0 = 3 };
 
 struct FwdParams {
   LvsaRows x, y, h, n;
@@ -39,51 +40,6 @@ struct FwdParams {
   float alpha, eps, post_eps;
   float2 *stats, *post_stats;
 };
-
-// Vectors of channels in shared memory, `pitch` floats each.  Of 8 values the
-// first and last four lie half a vector apart, so that the lanes of a warp
-// touch consecutive 16 bytes.
-enum { kA = 0, kB = 1, kG1 = 2, kG0 = 3 };
-
-template <int VEC>
-struct SharedVector {
-  static constexpr int kQuads = VEC == 1 ? 1 : VEC / 4;
-  using Q = typename std::conditional<VEC == 1, float, float4>::type;
-  Q* quad[kQuads];  // this thread's first
-
-  __device__ __forceinline__ SharedVector(float* all, int pitch, int which, int column) {
-#pragma unroll
-    for (int j = 0; j < kQuads; ++j)
-      quad[j] = reinterpret_cast<Q*>(all + which * pitch + j * (pitch / kQuads)) + column / VEC;
-  }
-  // At `vectors` (a constant) from the first.
-  __device__ __forceinline__ void get(int vectors, float (&f)[VEC]) const {
-    if constexpr (VEC == 1) {
-      f[0] = quad[0][vectors];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kQuads; ++j) {
-        const float4 q = quad[j][vectors];
-        f[4 * j] = q.x; f[4 * j + 1] = q.y; f[4 * j + 2] = q.z; f[4 * j + 3] = q.w;
-      }
-    }
-  }
-  __device__ __forceinline__ void put(const float (&f)[VEC]) const {
-    if constexpr (VEC == 1) {
-      quad[0][0] = f[0];
-    } else {
-#pragma unroll
-      for (int j = 0; j < kQuads; ++j) quad[j][0] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-    }
-  }
-};
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
-}
 
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
 template <typename TS, typename TB, int FORM, int VEC, int K>
@@ -129,20 +85,20 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
         vector_or<VEC>(p.v.shift, b, f, c, 0.f, m);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o[e] += m[e];
-        SharedVector<VEC>(held, pitch, kA, c).put(w);
-        SharedVector<VEC>(held, pitch, kB, c).put(o);
+        SharedVector<VEC>(held, pitch, kA, c).put(0, w);
+        SharedVector<VEC>(held, pitch, kB, c).put(0, o);
       }
       if constexpr (JOIN) {
         vector_or<VEC>(p.v.gate, b, f, c, 1.f, m);
         vector_or<VEC>(p.v.post_weight, 0, 0, c, 1.f, w);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[e] *= m[e];
-        SharedVector<VEC>(held, pitch, kG1, c).put(w);
+        SharedVector<VEC>(held, pitch, kG1, c).put(0, w);
         if (g0) {
           vector_or<VEC>(p.v.post_bias, 0, 0, c, 0.f, o);
 #pragma unroll
           for (int e = 0; e < VEC; ++e) o[e] *= m[e];
-          SharedVector<VEC>(held, pitch, kG0, c).put(o);
+          SharedVector<VEC>(held, pitch, kG0, c).put(0, o);
         }
       }
     }
@@ -192,7 +148,7 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
     if (start + mine < end) fetch();
     for (uint32_t row = start + mine; row < end; row += teams) {
       float z[K][VEC];
-      if constexpr (RING) asm volatile("cp.async.wait_all;" ::: "memory");
+      if constexpr (RING) copy_async_wait();
       if constexpr (JOIN) {
         float2 st = make_float2(0.f, 1.f);
         if constexpr (POST) {

@@ -9,8 +9,9 @@
 // The forward's h is computed again from x and y rather than read: the same
 // bytes, and its rounding to the stream's type does not enter the gradients.
 //
-// A CTA walks consecutive rows and a thread owns fixed columns, so P, Q, P2
-// and Q2 are sums in its registers.  At the end of a group that lies within
+// A CTA walks consecutive rows, the next one on its way into shared memory
+// (cp.async, each thread's own part), and a thread owns fixed columns, so P,
+// Q, P2 and Q2 are sums in its registers.  At the end of a group that lies within
 // one CTA they give the gradients at once; a group that several CTAs share
 // goes through the workspace (at most two such pieces a CTA: its first and
 // its last), as do the sums over groups (one row a CTA), and a second kernel
@@ -25,113 +26,131 @@ namespace lvsa {
 namespace {
 
 // What the workspace holds, in floats:
-//   piece [2 * CTA + (not its first)][kPieceSums][width]: P, Q, P2, Q2
-//   total [CTA][kTotals][width]: dw, db, dw2, db2
-constexpr int kPieceSums = 4, kTotals = 4;
+//   piece [2 * CTA + (not its first)][4][width]: P, Q, P2, Q2
+//   total [CTA][4][width]: dw, db, dw2, db2
+constexpr int kSums = 4;
+enum { kA = 0, kG1 = 1, kG0 = 2 };  // the vectors held
 
 struct BwdParams {
   LvsaBlockNormGrad g;
   Vectors v;
   FastDiv by_seq, by_group;
-  uint32_t rows;
-  int32_t ctas;
+  uint32_t rows, groups;
+  int32_t ctas, piece_sums, total_sums;  // bits of the sums that are wanted
   float* pieces;
   float* totals;
 };
 
 // What a group's sums give at column c; b, f: the group's.
-__device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t b, int64_t f, int c, float P, float Q,
-                                            float P2, float Q2) {
+__device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t b, int64_t f, int c, const float (&q)[kSums]) {
   const LvsaBlockNorm& a = g.f;
   const int64_t at = (b * a.frames + f) * a.width + c;
-  if (g.dshift.ptr) any_store(g.dshift.ptr, g.dshift.dtype, at, Q);
+  if (g.dshift.ptr) any_store(g.dshift.ptr, g.dshift.dtype, at, q[1]);
   if (g.dscale.ptr) {
     const float w = a.next.weight ? any_load(a.next.weight, a.next.weight_dtype, c) : 1.f;
     const float o = a.next.bias ? any_load(a.next.bias, a.next.bias_dtype, c) : 0.f;
-    any_store(g.dscale.ptr, g.dscale.dtype, at, w * P + o * Q);
+    any_store(g.dscale.ptr, g.dscale.dtype, at, w * q[0] + o * q[1]);
   }
   if (g.dgate.ptr) {
     const float w = a.post.weight ? any_load(a.post.weight, a.post.weight_dtype, c) : 1.f;
     const float o = a.post.bias ? any_load(a.post.bias, a.post.bias_dtype, c) : 0.f;
-    any_store(g.dgate.ptr, g.dgate.dtype, at, w * P2 + o * Q2);
+    any_store(g.dgate.ptr, g.dgate.dtype, at, w * q[2] + o * q[3]);
   }
 }
 
-// The rows that a thread has asked for: x and dn (next norm), y (join), dh.
-template <typename TS, typename TB, bool JOIN, int VEC, int K>
-struct Fetched {
-  Pack<TS, VEC> x[K], dh[JOIN ? K : 1];
-  Pack<TB, VEC> dn[K], y[JOIN ? K : 1];
-};
-
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
-template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1) block_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
-  constexpr bool JOIN = FORM > 0, POST = FORM == 2;
+template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
+  constexpr bool JOIN = FORM > 0, POST = FORM == 2, RING = VEC > 1;
   __shared__ float2 slots[2 * kMaxWarps];
+  extern __shared__ float4 dynamic[];
+  float* const held = reinterpret_cast<float*>(dynamic);
   Team team(slots, blockDim.x >> 5);
   const LvsaBlockNormGrad& g = p.g;
   const LvsaBlockNorm& a = g.f;
   const Columns<VEC, K> col(team, a.width);
+  const int pitch = shared_pitch(a.width);
   const float inv = 1.f / static_cast<float>(a.width);
   const uint32_t r0 = static_cast<uint32_t>(first_row(p.rows, blockIdx.x, p.ctas));
   const uint32_t r1 = static_cast<uint32_t>(first_row(p.rows, blockIdx.x + 1, p.ctas));
-  const bool next = g.dn.ptr;
+  const bool next = g.dn.ptr, more = JOIN && g.dh.ptr;
 
-  // A, G1 and G0 of this thread's columns, [3][K][threads][VEC]: read and
-  // written by their own thread alone, so that no barrier is due.
-  extern __shared__ float4 held[];
-  constexpr int E = VEC > 4 ? 4 : VEC;
-  auto held_at = [&](int which, int k, int j) {
-    return reinterpret_cast<float*>(held) + (((which * K + k) * (VEC / E) + j) * static_cast<int>(blockDim.x) + threadIdx.x) * E;
-  };
-  auto hold = [&](int which, int k, const float (&q)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC / E; ++j) {
-      float part[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) part[e] = q[j * E + e];
-      Pack<float, E>::store(held_at(which, k, j), part);
-    }
-  };
-  auto recall = [&](int which, int k, float (&q)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC / E; ++j) {
-      using R = typename Pack<float, E>::R;
-      Pack<float, E> part;
-      float o[E];
-      part.u = *reinterpret_cast<const R*>(held_at(which, k, j));
-      part.get(o);
-#pragma unroll
-      for (int e = 0; e < E; ++e) q[j * E + e] = o[e];
-    }
-  };
-  float P[K][VEC], Q[K][VEC], P2[JOIN ? K : 1][VEC], Q2[POST ? K : 1][VEC];
-  bool first_total = true;
-  uint32_t group_end = 0;
-  int64_t b = 0, f = 0;
-  uint32_t group_start = 0;
+  // A, G1 and G0 of this thread's columns, and its part of the next row: read
+  // and written by their own thread alone, so that no barrier is due.
+  const SharedVector<VEC> A(held, pitch, kA, col.first), G1(held, pitch, JOIN ? kG1 : 0, col.first),
+      G0(held, pitch, POST ? kG0 : 0, col.first);
+  using PS = Pack<TS, VEC>;
+  using PB = Pack<TB, VEC>;
+  typename PS::R* const xs = reinterpret_cast<typename PS::R*>(held + (FORM + 1) * pitch) + threadIdx.x;
+  typename PS::R* const hs = xs + K * blockDim.x;
+  typename PB::R* const ns = reinterpret_cast<typename PB::R*>(hs - threadIdx.x + (JOIN ? K * blockDim.x : 0)) + threadIdx.x;
+  typename PB::R* const ys = ns + K * blockDim.x;
+  PS xr[RING ? 1 : K], hr[RING || !JOIN ? 1 : K];  // the row itself where nothing can be copied ahead
+  PB nr[RING ? 1 : K], yr[RING || !JOIN ? 1 : K];
 
-  Fetched<TS, TB, JOIN, VEC, K> in;
-  auto fetch = [&](uint32_t row) {
-    const uint32_t fb = p.by_seq.div(row);
-    const int64_t t = row - fb * p.by_seq.d;
+  const TS *x = nullptr, *dh = nullptr;
+  const TB *y = nullptr, *dn = nullptr;
+  uint32_t ahead = r0, ahead_end = r0;  // the row that fetch() takes, and where its sequence ends
+  float2 st_ahead = make_float2(0.f, 1.f), ps_ahead = st_ahead;
+  auto fetch = [&]() {
+    if (ahead == ahead_end) {
+      const uint32_t fb = p.by_seq.div(ahead);
+      const int64_t t = ahead - fb * p.by_seq.d;
+      ahead_end = (fb + 1) * p.by_seq.d;
+      x = static_cast<const TS*>(a.x.ptr) + fb * a.x.stride_b + t * a.x.stride_t + col.first;
+      dn = static_cast<const TB*>(g.dn.ptr) + fb * g.dn.stride_b + t * g.dn.stride_t + col.first;
+      if constexpr (JOIN) {
+        y = static_cast<const TB*>(a.y.ptr) + fb * a.y.stride_b + t * a.y.stride_t + col.first;
+        dh = static_cast<const TS*>(g.dh.ptr) + fb * g.dh.stride_b + t * g.dh.stride_t + col.first;
+      }
+    }
+    if (next) st_ahead = __ldg(reinterpret_cast<const float2*>(a.stats) + ahead);
+    if constexpr (POST) ps_ahead = __ldg(reinterpret_cast<const float2*>(a.post_stats) + ahead);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!col.in(k)) continue;
-      if (next) {
-        in.x[k].load(static_cast<const TS*>(a.x.ptr) + fb * a.x.stride_b + t * a.x.stride_t + col.at(k));
-        in.dn[k].load(static_cast<const TB*>(g.dn.ptr) + fb * g.dn.stride_b + t * g.dn.stride_t + col.at(k));
-      }
-      if constexpr (JOIN) {
-        in.y[k].load(static_cast<const TB*>(a.y.ptr) + fb * a.y.stride_b + t * a.y.stride_t + col.at(k));
-        if (g.dh.ptr) in.dh[k].load(static_cast<const TS*>(g.dh.ptr) + fb * g.dh.stride_b + t * g.dh.stride_t + col.at(k));
+      if constexpr (RING) {
+        if (next) {
+          copy_async<sizeof(xs[0])>(xs + k * blockDim.x, x + k * col.kStep);
+          copy_async<sizeof(ns[0])>(ns + k * blockDim.x, dn + k * col.kStep);
+        }
+        if constexpr (JOIN) {
+          copy_async<sizeof(ys[0])>(ys + k * blockDim.x, y + k * col.kStep);
+          if (more) copy_async<sizeof(hs[0])>(hs + k * blockDim.x, dh + k * col.kStep);
+        }
+      } else {
+        if (next) {
+          xr[k].load(x + k * col.kStep);
+          nr[k].load(dn + k * col.kStep);
+        }
+        if constexpr (JOIN) {
+          yr[k].load(y + k * col.kStep);
+          if (more) hr[k].load(dh + k * col.kStep);
+        }
       }
     }
+    ++ahead;
+    x += a.x.stride_t;
+    dn += g.dn.stride_t;
+    if constexpr (JOIN) {
+      y += a.y.stride_t;
+      dh += g.dh.stride_t;
+    }
+  };
+  auto take = [&](auto& row, const auto* slot, int k, float(&f)[VEC]) {
+    if constexpr (RING) row[0].u = slot[k * blockDim.x];
+    row[RING ? 0 : k].get(f);
   };
 
+  float P[K][VEC], Q[K][VEC], P2[JOIN ? K : 1][VEC], Q2[POST ? K : 1][VEC];
+  bool first_total = true;
+  uint32_t group_start = 0, group_end = 0, seq_end = r0;
+  int64_t b = 0, f = 0;
+  TS* dx = nullptr;
+  TB* dy = nullptr;
+  if (RING) fetch();
   for (uint32_t row = r0; row < r1; ++row) {
-    fetch(row);
+    if (!RING) fetch();
     if (row >= group_end) {  // a new group (or the first row)
       const uint32_t group = p.by_group.div(row);
       group_start = group * p.by_group.d;
@@ -152,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, 1) block_norm_bwd_kernel(const __grid
         vector_or<VEC>(p.v.scale, b, f, col.at(k), 0.f, m);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) w[e] *= 1.f + m[e];
-        hold(0, k, w);
+        A.put(32 * k, w);
         if constexpr (JOIN) {
           vector_or<VEC>(p.v.gate, b, f, col.at(k), 1.f, m);
           if constexpr (POST) {
@@ -164,106 +183,99 @@ __global__ void __launch_bounds__(THREADS, 1) block_norm_bwd_kernel(const __grid
               o[e] *= m[e];
               m[e] *= w[e];
             }
-            hold(2, k, o);
+            G0.put(32 * k, o);
           }
-          hold(1, k, m);
+          G1.put(32 * k, m);
         }
       }
     }
-    const int64_t t = row - b * p.by_seq.d;
+    if (row >= seq_end) {
+      const int64_t t = row - b * p.by_seq.d;
+      seq_end = static_cast<uint32_t>(b + 1) * p.by_seq.d;
+      dx = static_cast<TS*>(g.dx.ptr) + b * g.dx.stride_b + t * g.dx.stride_t + col.first;
+      if constexpr (JOIN) dy = static_cast<TB*>(g.dy.ptr) + b * g.dy.stride_b + t * g.dy.stride_t + col.first;
+    }
+    if constexpr (RING) copy_async_wait();
+    const float2 st = st_ahead, ps = ps_ahead;
     // d: gradient of z, yh: yhat.  Columns outside the row stay zero.
-    float d[K][VEC], yh[JOIN ? K : 1][VEC];
-    float2 ps = make_float2(0.f, 1.f);
-    if constexpr (POST) ps = __ldg(reinterpret_cast<const float2*>(a.post_stats) + row);
+    float d[K][VEC], yh[JOIN ? K : 1][VEC], zh[K][VEC], v[K][VEC];
+    float s = 0.f, sz = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
+        d[k][e] = zh[k][e] = v[k][e] = 0.f;
         if constexpr (JOIN) yh[k][e] = 0.f;
       }
+      if (!col.in(k)) continue;
       if constexpr (JOIN) {
-        if (col.in(k)) {
-          in.y[k].get(yh[k]);
-          if constexpr (POST) {
+        take(yr, ys, k, yh[k]);
+        if (more) take(hr, hs, k, d[k]);
+        if constexpr (POST) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) yh[k][e] = (yh[k][e] - ps.x) * ps.y;
-          }
+          for (int e = 0; e < VEC; ++e) yh[k][e] = (yh[k][e] - ps.x) * ps.y;
         }
+      }
+      if (!next) continue;
+      take(xr, xs, k, zh[k]);
+      take(nr, ns, k, v[k]);
+      float q[VEC];
+      if constexpr (JOIN) {
+        G1.get(32 * k, q);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) zh[k][e] = a.residual_scale * zh[k][e] + yh[k][e] * q[e];
+      }
+      if constexpr (POST) {
+        G0.get(32 * k, q);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) zh[k][e] += q[e];
+      }
+      A.get(32 * k, q);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        zh[k][e] = (zh[k][e] - st.x) * st.y;
+        P[k][e] += v[k][e] * zh[k][e];
+        Q[k][e] += v[k][e];
+        v[k][e] *= q[e];
+        s += v[k][e];
+        sz += v[k][e] * zh[k][e];
       }
     }
-    auto start_d = [&]() {
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) d[k][e] = 0.f;
-        if constexpr (JOIN)
-          if (g.dh.ptr && col.in(k)) in.dh[k].get(d[k]);
-      }
-    };
+    if (RING && row + 1 < r1) fetch();
     if (next) {
-      const float2 st = __ldg(reinterpret_cast<const float2*>(a.stats) + row);
-      float zh[K][VEC], v[K][VEC];
-      float s = 0.f, sz = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zh[k][e] = v[k][e] = 0.f;
-        if (!col.in(k)) continue;
-        in.x[k].get(zh[k]);
-        in.dn[k].get(v[k]);
-        float A[VEC], G1[VEC], G0[VEC];
-        recall(0, k, A);
-        if constexpr (JOIN) recall(1, k, G1);
-        if constexpr (POST) recall(2, k, G0);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          float z = zh[k][e];
-          if constexpr (POST) z = a.residual_scale * z + (yh[k][e] * G1[e] + G0[e]);
-          else if constexpr (JOIN) z = a.residual_scale * z + yh[k][e] * G1[e];
-          z = (z - st.x) * st.y;
-          P[k][e] += v[k][e] * z;
-          Q[k][e] += v[k][e];
-          zh[k][e] = z;
-          v[k][e] *= A[e];
-          s += v[k][e];
-          sz += v[k][e] * z;
-        }
-      }
       const float2 m = team.sum2(s, sz);
       const float m0 = a.next.kind == LVSA_BLOCK_NORM_LAYER ? m.x * inv : 0.f, m1 = m.y * inv;
-      start_d();
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (col.in(k)) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[k][e] += st.y * (v[k][e] - m0 - zh[k][e] * m1);
+          for (int e = 0; e < VEC; ++e) d[k][e] += st.y * ((v[k][e] - m0) - zh[k][e] * m1);
         }
-    } else {
-      start_d();
     }
     if (g.dx.ptr) {
-      TS* dx = static_cast<TS*>(g.dx.ptr) + b * g.dx.stride_b + t * g.dx.stride_t;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!col.in(k)) continue;
         float o[VEC];
 #pragma unroll
         for (int e = 0; e < VEC; ++e) o[e] = JOIN ? a.residual_scale * d[k][e] : d[k][e];
-        Pack<TS, VEC>::store(dx + col.at(k), o);
+        PS::store(dx + k * col.kStep, o);
       }
+      dx += g.dx.stride_t;
     }
     if constexpr (JOIN) {
-      float s = 0.f, sy = 0.f;
+      float sy = 0.f;
+      s = 0.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!col.in(k)) continue;
-        float G1[VEC];
-        recall(1, k, G1);
+        float q[VEC];
+        G1.get(32 * k, q);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           P2[k][e] += d[k][e] * yh[k][e];
           if constexpr (POST) Q2[k][e] += d[k][e];
-          d[k][e] *= G1[e];
+          d[k][e] *= q[e];
           if constexpr (POST) {
             s += d[k][e];
             sy += d[k][e] * yh[k][e];
@@ -277,98 +289,102 @@ __global__ void __launch_bounds__(THREADS, 1) block_norm_bwd_kernel(const __grid
           m0 = a.post.kind == LVSA_BLOCK_NORM_LAYER ? m.x * inv : 0.f;
           m1 = m.y * inv;
         }
-        TB* dy = static_cast<TB*>(g.dy.ptr) + b * g.dy.stride_b + t * g.dy.stride_t;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!col.in(k)) continue;
-          float o[VEC];
+          if constexpr (POST) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            if constexpr (POST) o[e] = ps.y * (d[k][e] - m0 - yh[k][e] * m1);
-            else o[e] = d[k][e];
+            for (int e = 0; e < VEC; ++e) d[k][e] = ps.y * ((d[k][e] - m0) - yh[k][e] * m1);
           }
-          Pack<TB, VEC>::store(dy + col.at(k), o);
+          PB::store(dy + k * col.kStep, d[k]);
         }
+        dy += g.dy.stride_t;
       }
     }
+    if (row + 1 < r1 && row + 1 < group_end) continue;
+
     // End of this CTA's part of the group.
-    if (row + 1 == r1 || row + 1 == group_end) {
-      const bool whole = r0 <= group_start && r1 >= group_end;
-      float* piece = p.pieces + (2 * static_cast<int64_t>(blockIdx.x) + (r0 < group_start ? 1 : 0)) * kPieceSums * a.width;
-      float* total = p.totals + static_cast<int64_t>(blockIdx.x) * kTotals * a.width;
+    const bool whole = r0 <= group_start && r1 >= group_end;
+    float* piece = p.pieces + (2 * static_cast<int64_t>(blockIdx.x) + (r0 < group_start ? 1 : 0)) * kSums * a.width;
+    float* total = p.totals + static_cast<int64_t>(blockIdx.x) * kSums * a.width;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (!col.in(k)) continue;
+    for (int k = 0; k < K; ++k) {
+      if (!col.in(k)) continue;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int c = col.at(k) + e;
-          float q[4] = {P[k][e], Q[k][e], 0.f, 0.f};
-          if constexpr (JOIN) q[2] = P2[k][e];
-          if constexpr (POST) q[3] = Q2[k][e];
-          if (whole) {
-            store_group(g, b, f, c, q[0], q[1], q[2], q[3]);
-          } else {
+      for (int e = 0; e < VEC; ++e) {
+        const int c = col.at(k) + e;
+        float q[kSums] = {P[k][e], Q[k][e], 0.f, 0.f};
+        if constexpr (JOIN) q[2] = P2[k][e];
+        if constexpr (POST) q[3] = Q2[k][e];
+        if (whole) {
+          store_group(g, b, f, c, q);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) piece[i * a.width + c] = q[i];
-          }
-          if (p.totals) {
-            const int64_t fs = b * a.scale.stride_b + f * a.scale.stride_f + c, fg = b * a.gate.stride_b + f * a.gate.stride_f + c;
-            const float up = a.scale.ptr ? 1.f + any_load(a.scale.ptr, a.scale.dtype, fs) : 1.f;
-            const float gt = a.gate.ptr ? any_load(a.gate.ptr, a.gate.dtype, fg) : 1.f;
-            const float add[4] = {up * q[0], up * q[1], gt * q[2], gt * q[3]};
+          for (int i = 0; i < kSums; ++i)
+            if (p.piece_sums >> i & 1) piece[i * a.width + c] = q[i];
+        }
+        if (p.total_sums) {
+          const int64_t fs = b * a.scale.stride_b + f * a.scale.stride_f + c, fg = b * a.gate.stride_b + f * a.gate.stride_f + c;
+          const float up = a.scale.ptr ? 1.f + any_load(a.scale.ptr, a.scale.dtype, fs) : 1.f;
+          const float gt = a.gate.ptr ? any_load(a.gate.ptr, a.gate.dtype, fg) : 1.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) total[i * a.width + c] = add[i] + (first_total ? 0.f : total[i * a.width + c]);
-          }
+          for (int i = 0; i < kSums; ++i)
+            if (p.total_sums >> i & 1)
+              total[i * a.width + c] = (i < 2 ? up : gt) * q[i] + (first_total ? 0.f : total[i * a.width + c]);
         }
       }
-      first_total = false;
     }
+    first_total = false;
   }
 }
 
 // Adds what the CTAs left in the workspace: blockIdx.y = 0 the totals, k > 0
-// the group that the boundary between CTAs k - 1 and k lies in, once a group.
-// A block takes 32 columns; its rows of threads share the CTAs and are added
-// in order.
-constexpr int kJoinRows = 16;
+// the k-th group, or, with more groups than CTAs, the group that the boundary
+// between CTAs k - 1 and k cuts; a group that no boundary cuts is done.  A
+// block takes 32 columns; its rows of threads share the CTAs and are added in
+// order.
+constexpr int kJoinRows = 32;
 __global__ void __launch_bounds__(32 * kJoinRows) block_norm_sums_kernel(const __grid_constant__ BwdParams p) {
   const LvsaBlockNorm& a = p.g.f;
   const int c = blockIdx.x * 32 + threadIdx.x;
-  int64_t first = 0, last = p.ctas;  // CTAs whose rows are added
-  int64_t group = -1;
-  if (blockIdx.y == 0) {
-    if (!p.totals) return;
-  } else {
-    const int64_t r = first_row(p.rows, blockIdx.y, p.ctas);
-    group = p.by_group.div(static_cast<uint32_t>(r));
-    const int64_t g0 = group * p.by_group.d, g1 = g0 + p.by_group.d;
-    first = static_cast<int64_t>(blockIdx.y) - 1;
-    if (r == g0 || first_row(p.rows, first, p.ctas) > g0) return;  // no group is cut here, or another block's
-    last = row_owner(p.rows, g1 - 1, p.ctas) + 1;
+  int64_t first = 0, last = p.ctas, group = -1, start = 0;  // CTAs whose sums are added
+  int wanted = p.total_sums;
+  if (blockIdx.y > 0) {
+    wanted = p.piece_sums;
+    const int64_t cut = p.groups <= static_cast<uint32_t>(p.ctas) ? 0 : first_row(p.rows, blockIdx.y, p.ctas);
+    group = cut ? p.by_group.div(static_cast<uint32_t>(cut)) : blockIdx.y - 1;
+    start = group * p.by_group.d;
+    first = row_owner(p.rows, start, p.ctas);
+    last = row_owner(p.rows, start + p.by_group.d - 1, p.ctas) + 1;
+    // Whole groups are done; of several cuts the first one's block is here.
+    if (last - first == 1 || (cut && (cut == start || blockIdx.y != first + 1))) return;
   }
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (!wanted) return;
+  float sum[kSums] = {0.f, 0.f, 0.f, 0.f};
   if (c < a.width) {
+#pragma unroll 4
     for (int64_t i = first + threadIdx.y; i < last; i += kJoinRows) {
-      const float* from = p.totals + i * kTotals * a.width;
+      const float* from = p.totals + i * kSums * a.width;
       if (group >= 0) {
-        const bool later = first_row(p.rows, i, p.ctas) < group * p.by_group.d;  // the group is not its CTA's first
-        from = p.pieces + (2 * i + later) * kPieceSums * a.width;
+        const bool later = first_row(p.rows, i, p.ctas) < start;  // the group is not its CTA's first
+        from = p.pieces + (2 * i + later) * kSums * a.width;
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] += from[j * a.width + c];
+      for (int j = 0; j < kSums; ++j)
+        if (wanted >> j & 1) sum[j] += from[j * a.width + c];
     }
   }
-  __shared__ float part[4][kJoinRows][32];
+  __shared__ float part[kSums][kJoinRows][32];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) part[j][threadIdx.y][threadIdx.x] = sum[j];
+  for (int j = 0; j < kSums; ++j) part[j][threadIdx.y][threadIdx.x] = sum[j];
   __syncthreads();
   if (threadIdx.y != 0 || c >= a.width) return;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < kSums; ++j)
     for (int i = 1; i < kJoinRows; ++i) sum[j] += part[j][i][threadIdx.x];
   if (group >= 0) {
     const int64_t b = group / a.frames;
-    store_group(p.g, b, group - b * a.frames, c, sum[0], sum[1], sum[2], sum[3]);
+    store_group(p.g, b, group - b * a.frames, c, sum);
     return;
   }
   if (p.g.dweight) any_store(p.g.dweight, a.next.weight_dtype, c, sum[0]);
@@ -377,34 +393,47 @@ __global__ void __launch_bounds__(32 * kJoinRows) block_norm_sums_kernel(const _
   if (p.g.dpost_bias) any_store(p.g.dpost_bias, a.post.bias_dtype, c, sum[3]);
 }
 
-inline bool any_total(const LvsaBlockNormGrad& g) { return g.dweight || g.dbias || g.dpost_weight || g.dpost_bias; }
+inline int piece_sums(const LvsaBlockNormGrad& g) {
+  const LvsaBlockNorm& a = g.f;
+  return (g.dscale.ptr ? 1 : 0) | (g.dshift.ptr || (g.dscale.ptr && a.next.bias) ? 2 : 0) | (g.dgate.ptr ? 4 : 0) |
+         (g.dgate.ptr && a.post.bias ? 8 : 0);
+}
+inline int total_sums(const LvsaBlockNormGrad& g) {
+  return (g.dweight ? 1 : 0) | (g.dbias ? 2 : 0) | (g.dpost_weight ? 4 : 0) | (g.dpost_bias ? 8 : 0);
+}
 
 // CTAs of the launch, or the launch itself (workspace known by then).
-template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS>
+template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS, int CTAS>
 int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cudaStream_t s) {
-  auto kern = block_norm_bwd_kernel<TS, TB, FORM, VEC, K, THREADS>;
+  auto kern = block_norm_bwd_kernel<TS, TB, FORM, VEC, K, THREADS, CTAS>;
   const int vectors = (g.f.width + VEC - 1) / VEC;
   const int threads = ((vectors + K - 1) / K + 31) / 32 * 32;
   static std::atomic<uint64_t> last{0};
   const int64_t rows = static_cast<int64_t>(g.f.batch) * g.f.seq;
-  const int shared = (FORM + 1) * threads * VEC * K * static_cast<int>(sizeof(float));
-  const int64_t ctas = std::min<int64_t>(rows, resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last));
+  const int shared = (FORM + 1) * shared_pitch(g.f.width) * static_cast<int>(sizeof(float)) +
+                     (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
+  int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
+  // A CTA ends with a piece of sums the size of some rows: not fewer than 8 rows each, unless SMs are left over.
+  ctas = std::min(ctas, std::max<int64_t>(rows / 8, std::min<int64_t>(rows, device_sms())));
   if (ctas_only) {
     *ctas_only = ctas;
     return LVSA_OK;
   }
   float* space = static_cast<float*>(g.workspace);
+  const int64_t groups = static_cast<int64_t>(g.f.batch) * g.f.frames;
   const BwdParams p{g, v, FastDiv(g.f.seq), FastDiv(g.f.seq / g.f.frames), static_cast<uint32_t>(rows),
-                    static_cast<int32_t>(ctas), space,
-                    any_total(g) ? space + ctas * 2 * kPieceSums * g.f.width : nullptr};
+                    static_cast<uint32_t>(groups), static_cast<int32_t>(ctas), piece_sums(g), total_sums(g), space,
+                    space + ctas * 2 * kSums * g.f.width};
   kern<<<p.ctas, threads, shared, s>>>(p);
   if (cudaGetLastError() != cudaSuccess) return LVSA_ERR_CUDA;
-  block_norm_sums_kernel<<<dim3((g.f.width + 31) / 32, p.ctas), dim3(32, kJoinRows), 0, s>>>(p);
+  if (!p.piece_sums && !p.total_sums) return LVSA_OK;
+  const dim3 grid((g.f.width + 31) / 32, static_cast<unsigned>(groups <= ctas ? groups + 1 : ctas));
+  block_norm_sums_kernel<<<grid, dim3(32, kJoinRows), 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-// 8 columns a thread up to 5376 channels, 16 beyond; the fewer threads a CTA
+// 8 columns a thread up to 5120 channels, 16 beyond; the fewer threads a CTA
 // may have, the more registers they get.  Value by value where the accesses
 // of a vector do not fit.
 template <typename TS, typename TB, int FORM>
@@ -414,10 +443,10 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   const int width = g.f.width;
   if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
       !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC))
-    return launch<TS, TB, FORM, 1, 16, 512>(g, v, ctas, s);
-  if (width <= 8 * 384) return launch<TS, TB, FORM, VEC, 8 / VEC, 384>(g, v, ctas, s);
-  if (width <= 8 * 672) return launch<TS, TB, FORM, VEC, 8 / VEC, 672>(g, v, ctas, s);
-  return launch<TS, TB, FORM, VEC, 16 / VEC, 512>(g, v, ctas, s);
+    return launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
+  if (width <= 8 * 256) return launch<TS, TB, FORM, VEC, 8 / VEC, 256, FORM ? 2 : 3>(g, v, ctas, s);
+  if (width <= 8 * 640) return launch<TS, TB, FORM, VEC, 8 / VEC, 640, 1>(g, v, ctas, s);
+  return launch<TS, TB, FORM, VEC, 16 / VEC, 512, 1>(g, v, ctas, s);
 }
 
 template <typename TS, typename TB>
@@ -451,7 +480,7 @@ int dispatch(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
 int workspace(const LvsaBlockNormGrad& g, int64_t* bytes) {
   int64_t ctas = 0;
   const int st = dispatch(g, &ctas, nullptr);
-  *bytes = ctas * g.f.width * (2 * kPieceSums + (any_total(g) ? kTotals : 0)) * static_cast<int64_t>(sizeof(float));
+  *bytes = ctas * g.f.width * (2 + (total_sums(g) ? 1 : 0)) * kSums * static_cast<int64_t>(sizeof(float));
   return st;
 }
 

@@ -214,6 +214,54 @@ struct Columns {
   }
 };
 
+__host__ __device__ inline int shared_pitch(int width) { return (width + 7) & ~7; }
+// Vectors of channels in shared memory, `pitch` floats each.  Of 8 values the
+// first and last four lie half a vector apart, so that the lanes of a warp
+// touch consecutive 16 bytes.
+template <int VEC>
+struct SharedVector {
+  static constexpr int kQuads = VEC == 1 ? 1 : VEC / 4;
+  using Q = typename std::conditional<VEC == 1, float, float4>::type;
+  Q* quad[kQuads];  // this thread's first
+
+  __device__ __forceinline__ SharedVector(float* all, int pitch, int which, int column) {
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+      quad[j] = reinterpret_cast<Q*>(all + which * pitch + j * (pitch / kQuads)) + column / VEC;
+  }
+  // At `vectors` (a constant) from the first.
+  __device__ __forceinline__ void get(int vectors, float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      f[0] = quad[0][vectors];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) {
+        const float4 q = quad[j][vectors];
+        f[4 * j] = q.x; f[4 * j + 1] = q.y; f[4 * j + 2] = q.z; f[4 * j + 3] = q.w;
+      }
+    }
+  }
+  __device__ __forceinline__ void put(int vectors, const float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      quad[0][vectors] = f[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kQuads; ++j) quad[j][vectors] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+    }
+  }
+};
+
+// An asynchronous copy of one vector into a thread's slot of shared memory; a
+// thread waits for its own copies only.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  const uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
+}
+
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // How many of a row's values each warp of a team holds (shared memory, filled
 // by every thread of the CTA with the same numbers) and this warp's reciprocal.
 struct Held {
