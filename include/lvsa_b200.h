@@ -362,6 +362,38 @@ typedef struct LvsaBlockNormGrad {
 int lvsa_block_norm_workspace(const LvsaBlockNormGrad* args, int64_t* bytes);
 int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
 
+/* ---- Linear with 4-bit weights and group scales, for few rows ----
+ * out[m, n] = sum_k act(x[m, k]) * scale[n, k / group] * code[n, k] (+ bias[n]),
+ * codes -8 .. 7.  For the Linears that see one row a sequence or a frame (the
+ * modulation of a diffusion transformer from its time embedding), whose time
+ * is their weights'.  No counterpart in the reference.
+ *
+ * lvsa_w4_pack lays codes [n, k] (int8, row stride ld) out once, into
+ * lvsa_w4_bytes bytes: tiles of 16 rows x 64 columns, 512 bytes each, the
+ * tiles of a row of tiles side by side; rows and columns past the end hold
+ * code 0.  `scales`: with T = ceil(k / 64) and words of two 2-byte scales (rows
+ * r and r + 8 of a tile), [ceil(n / 16)][ceil(k / group)][8] words for group 64
+ * or 128 and [ceil(n / 16)][T][8][2] words for group 32, 0 past the end.
+ *
+ * Products are exact (x as one to three bf16 parts, their number by what act
+ * and x's type need) and sums fp32; one rounding to the output's type.  A row
+ * of x that holds an infinity or NaN gives NaN. */
+enum { LVSA_W4_ACT_NONE = 0, LVSA_W4_ACT_SILU = 1 };
+typedef struct LvsaW4Linear {
+  const void* x;     /* [m, k], row stride ldx elements, bf16 / f16 / fp32       */
+  const void* tiles; /* from lvsa_w4_pack, 16-byte aligned                       */
+  const void* scales; /* 8-byte aligned                                          */
+  const void* bias;  /* [n] or NULL                                              */
+  void* out;         /* [m, n], row stride ldo elements                          */
+  int64_t ldx, ldo;
+  int32_t m, n, k, group; /* group 32, 64 or 128                                 */
+  int32_t x_dtype, out_dtype, bias_dtype, scale_dtype; /* scales bf16 or f16     */
+  int32_t activation; /* LVSA_W4_ACT_*                                           */
+} LvsaW4Linear;
+int lvsa_w4_bytes(int32_t n, int32_t k, int64_t* bytes);
+int lvsa_w4_pack(const int8_t* codes, int64_t ld, int32_t n, int32_t k, void* tiles, void* stream);
+int lvsa_w4_linear(const LvsaW4Linear* args, void* stream);
+
 /* Human-readable name of a status code. */
 const char* lvsa_status_str(int status);
 

@@ -28,7 +28,8 @@ LVSA_MAX_FRAMES = 2048
 
 EXPORTED_SYMBOLS = ("lvsa_mask_layout", "lvsa_build_mask", "lvsa_attn_fwd", "lvsa_quantize_e4m3",
                     "lvsa_attn_fwd_fp8", "lvsa_attn_fwd_fp8_noalloc", "lvsa_qk_prologue", "lvsa_copy_segments", "lvsa_out_proj", "lvsa_status_str",
-                    "lvsa_abi_version", "lvsa_block_norm_fwd", "lvsa_block_norm_workspace", "lvsa_block_norm_bwd")
+                    "lvsa_abi_version", "lvsa_block_norm_fwd", "lvsa_block_norm_workspace", "lvsa_block_norm_bwd",
+                    "lvsa_w4_bytes", "lvsa_w4_pack", "lvsa_w4_linear")
 LVSA_DTYPE_E4M3 = 2
 LVSA_DTYPE_F32 = 3
 LVSA_NORM_NONE, LVSA_NORM_RMS_ROW, LVSA_NORM_RMS_HEAD, LVSA_NORM_LAYER_HEAD = 0, 1, 2, 3
@@ -127,6 +128,15 @@ class LvsaBlockNormGrad(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", _i64)]
 
 
+LVSA_W4_ACT_NONE, LVSA_W4_ACT_SILU = 0, 1
+
+
+class LvsaW4Linear(ctypes.Structure):
+    _fields_ = [("x", _vp), ("tiles", _vp), ("scales", _vp), ("bias", _vp), ("out", _vp), ("ldx", _i64), ("ldo", _i64),
+                ("m", _i32), ("n", _i32), ("k", _i32), ("group", _i32), ("x_dtype", _i32), ("out_dtype", _i32),
+                ("bias_dtype", _i32), ("scale_dtype", _i32), ("activation", _i32)]
+
+
 class LvsaFp8Scales(ctypes.Structure):
     _fields_ = [(n, _vp) for n in ("q", "k", "v", "text_q", "text_k", "text_v", "v_ref")]
 
@@ -176,6 +186,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.lvsa_block_norm_workspace.restype = ctypes.c_int
         lib.lvsa_block_norm_bwd.argtypes = [ctypes.POINTER(LvsaBlockNormGrad), _vp]
         lib.lvsa_block_norm_bwd.restype = ctypes.c_int
+        lib.lvsa_w4_bytes.argtypes = [_i32, _i32, ctypes.POINTER(_i64)]
+        lib.lvsa_w4_bytes.restype = ctypes.c_int
+        lib.lvsa_w4_pack.argtypes = [_vp, _i64, _i32, _i32, _vp, _vp]
+        lib.lvsa_w4_pack.restype = ctypes.c_int
+        lib.lvsa_w4_linear.argtypes = [ctypes.POINTER(LvsaW4Linear), _vp]
+        lib.lvsa_w4_linear.restype = ctypes.c_int
         lib.lvsa_copy_segments.argtypes = [ctypes.POINTER(LvsaCopySegment), _i32, _i32, _vp]
         lib.lvsa_copy_segments.restype = ctypes.c_int
         lib.lvsa_status_str.argtypes = [ctypes.c_int]

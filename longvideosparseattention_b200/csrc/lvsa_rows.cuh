@@ -45,6 +45,7 @@ struct Pack {
   using R = typename Raw<static_cast<int>(sizeof(T)) * VEC>::type;
   R u;
   __device__ __forceinline__ void load(const T* p) { u = __ldg(reinterpret_cast<const R*>(p)); }
+  __device__ __forceinline__ void load_plain(const T* p) { u = *reinterpret_cast<const R*>(p); }
   __device__ __forceinline__ void get(float (&f)[VEC]) const {
     const T* h = reinterpret_cast<const T*>(&u);
 #pragma unroll
@@ -77,10 +78,13 @@ struct Vector {
   int32_t dtype;
 };
 
+// Plain loads, here and below: the toolkit's __ldg of a 16-bit float is an asm
+// statement without side effects, which the compiler may move above the test
+// that p is there (or in range) at all.
 __device__ __forceinline__ float any_load(const void* p, int32_t dtype, int64_t i) {
-  if (dtype == LVSA_DTYPE_F32) return __ldg(static_cast<const float*>(p) + i);
-  if (dtype == LVSA_DTYPE_BF16) return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + i));
-  return __half2float(__ldg(static_cast<const __half*>(p) + i));
+  if (dtype == LVSA_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == LVSA_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
 }
 __device__ __forceinline__ void any_store(void* p, int32_t dtype, int64_t i, float v) {
   if (dtype == LVSA_DTYPE_F32) static_cast<float*>(p)[i] = v;
@@ -97,14 +101,14 @@ __device__ __forceinline__ void any_load(const void* p, int32_t dtype, int64_t i
     for (int j = 0; j < VEC / E; ++j) {
       Pack<float, E> q;
       float g[E];
-      q.load(static_cast<const float*>(p) + i + j * E);
+      q.load_plain(static_cast<const float*>(p) + i + j * E);
       q.get(g);
 #pragma unroll
       for (int e = 0; e < E; ++e) f[j * E + e] = g[e];
     }
   } else {
     Pack<__half, VEC> q;  // the bits of either 16-bit type
-    q.load(static_cast<const __half*>(p) + i);
+    q.load_plain(static_cast<const __half*>(p) + i);
     if (dtype == LVSA_DTYPE_F16) {
       q.get(f);
     } else {

@@ -1,0 +1,351 @@
+// Linear with 4-bit weights and a scale for each group of columns, for few
+// rows of x: out[m, n] = sum_k act(x[m, k]) s[n, k / group] q[n, k] (+ bias).
+// Bound: HBM, n k / 2 bytes of codes and 2 n k / group of scales read once.
+//
+// Arithmetic.  A code q = -8 .. 7 is stored as u = q + 8, and the bf16 number
+// with u in the top of its mantissa is w = 1 + u / 16, made from u by a shift
+// and one three-input operation for two codes; q = 16 (w - 1.5).  So with
+// x's bf16 parts as the other operand of m16n8k16 (weights as its 16 rows,
+// parts of rows of x as its 8 columns; bf16 products are exact, sums fp32)
+//   sum of a group = 16 (sum_k x w - 1.5 sum_k x),
+// where the second sum belongs to x and the 16 waits until the end.  The
+// offset costs two to three bits of the fp32 sum (w is 1.5 where q / 16 is
+// 0.3 on average), a subtraction a code would cost a third of the issue slots.
+// x enters as bf16 parts: one where it is bf16 and no activation applies,
+// two for f16 and for an activation of a 16-bit x (16 bits), three for fp32
+// (24 bits).  With few rows the columns they take are free.
+//
+// Work.  A CTA an SM, 16 warps; a CTA takes rows of tiles (16 rows of
+// weights) in turn and its warps share a row's tiles of 64 columns, so that
+// even a narrow Linear keeps every SM reading.  Tiles come through a ring in
+// shared memory (cp.async, a thread's own 16 bytes: no barrier), which runs
+// on across rows of tiles while the warps' sums are joined.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "lvsa_rows.cuh"
+
+namespace lvsa {
+namespace {
+
+constexpr int kTileN = 16, kTileK = 64;
+constexpr int kWarpsW4 = 16, kThreadsW4 = 32 * kWarpsW4;
+constexpr int kDepth = 8;                      // tiles of a warp on their way
+constexpr int kMaxShared = 227 * 1024 - 1024;
+
+struct W4Params {
+  LvsaW4Linear a;
+  int32_t k_tiles, row_tiles, parts, pass_rows;  // rows of x a pass (blockIdx.y)
+  int32_t chunk_tiles;                           // k tiles of x held at once
+  int32_t pitch;                                 // bf16 values between the columns of x held
+};
+
+// ---- layout: lane l = 4 r + j of a tile holds rows r and r + 8, columns
+// 8 j .. 8 j + 7 and 32 + 8 j .. of it, as the four steps' A fragments.  Word
+// s: columns c = 32 (s / 2) + 8 j + 4 (s % 2) ..+3; register i = 0 .. 3 of the
+// fragment has row r + 8 (i & 1) and columns c + 2 (i >> 1), +1, whose codes
+// lie at bits 3 + 4 i (low half) and 19 + 4 i of the word (mod 32).
+__global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64_t ld, int n, int k, int k_tiles,
+                                                      int64_t total, uint4* tiles) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= total) return;
+  const int lane = at & 31, r = lane >> 2, j = lane & 3;
+  const int64_t tile = at >> 5, row0 = tile / k_tiles * kTileN;
+  const int col0 = static_cast<int>(tile % k_tiles) * kTileK;
+  uint32_t words[4];
+  for (int s = 0; s < 4; ++s) {
+    uint32_t w = 0;
+    for (int i = 0; i < 4; ++i)
+      for (int q = 0; q < 2; ++q) {
+        const int64_t row = row0 + r + 8 * (i & 1);
+        const int col = col0 + 32 * (s >> 1) + 8 * j + 4 * (s & 1) + 2 * (i >> 1) + q;
+        const int code = row < n && col < k ? codes[row * ld + col] : 0;
+        const uint32_t u = static_cast<uint32_t>(code + 8) & 15u;
+        w |= __funnelshift_l(u, u, 3 + 4 * i + 16 * q);  // a rotation: u has four bits
+      }
+    words[s] = w;
+  }
+  tiles[at] = make_uint4(words[0], words[1], words[2], words[3]);
+}
+
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
+// The A fragment of a word: 1 + u / 16 as bf16 pairs.
+__device__ __forceinline__ void weights(uint32_t w, uint32_t (&a)[4]) {
+  constexpr uint32_t kMask = 0x00780078u, kOne = 0x3f803f80u;
+  a[0] = (w & kMask) | kOne;
+  a[1] = ((w >> 4) & kMask) | kOne;
+  a[2] = ((w >> 8) & kMask) | kOne;
+  a[3] = (__funnelshift_r(w, w, 12) & kMask) | kOne;
+}
+
+template <int N>
+__device__ __forceinline__ void copy_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns.
+template <int NT, bool HALVES, typename TSc>
+__global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
+  using Word = typename std::conditional<HALVES, uint2, uint32_t>::type;
+  constexpr int kBlocks = HALVES ? 2 : 1;  // sums of x a k tile
+  constexpr int kCols = 8 * NT;
+  extern __shared__ uint4 shared_w4[];
+  uint4* const ring = shared_w4;                                                   // [depth][threads]
+  Word* const scale_ring = reinterpret_cast<Word*>(ring + kDepth * kThreadsW4);    // [depth][threads]
+  float* const joined = reinterpret_cast<float*>(scale_ring + kDepth * kThreadsW4);  // [warp][column][row]
+  float* const x_sums = joined + kWarpsW4 * kCols * kTileN;                        // [block][column]
+  __nv_bfloat16* const xs = reinterpret_cast<__nv_bfloat16*>(x_sums + p.chunk_tiles * kBlocks * kCols);  // [column][pitch]
+
+  const LvsaW4Linear& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
+  const int m0 = blockIdx.y * p.pass_rows, rows = min(p.pass_rows, a.m - m0), cols = rows * p.parts;
+
+  // This warp's tiles: warp, warp + 16, ... of every row of tiles that is the CTA's.
+  const int scale_words = HALVES ? p.k_tiles : (a.k + a.group - 1) / a.group;  // of a row of tiles, times 8
+  const int scale_shift = a.group == 128 ? 1 : 0;
+  int fetch_row = blockIdx.x, fetch_tile = warp, fetch_slot = threadIdx.x;
+  auto fetch = [&]() {
+    if (fetch_row < p.row_tiles && fetch_tile < p.k_tiles) {
+      const int64_t tile = static_cast<int64_t>(fetch_row) * p.k_tiles + fetch_tile;
+      copy_async<16>(ring + fetch_slot, static_cast<const uint4*>(a.tiles) + tile * 32 + lane);
+      copy_async<sizeof(Word)>(scale_ring + fetch_slot,
+                               static_cast<const Word*>(a.scales) +
+                                   (static_cast<int64_t>(fetch_row) * scale_words + (fetch_tile >> scale_shift)) * 8 + r);
+      fetch_slot += kThreadsW4;
+      if (fetch_slot >= kDepth * kThreadsW4) fetch_slot -= kDepth * kThreadsW4;
+      fetch_tile += kWarpsW4;
+      if (fetch_tile >= p.k_tiles) {
+        fetch_tile = warp;
+        fetch_row += gridDim.x;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) fetch();
+
+  // x's columns from k tile `first` on, as bf16 parts, and -1.5 times their
+  // sums: a thread takes 8 values, the threads of a block of columns add up.
+  auto stage = [&](int first) {
+    const int tiles = min(p.chunk_tiles, p.k_tiles - first), octets = tiles * (kTileK / 8);
+    constexpr int kLanes = HALVES ? 4 : 8;  // threads a block
+    for (int i = threadIdx.x; i < (rows * octets + 31) / 32 * 32; i += kThreadsW4) {
+      const int m = i / octets, o = i - m * octets;  // octets is a multiple of 8: a block lies in one row
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t k = static_cast<int64_t>(first) * kTileK + 8 * o + e;
+        v[e] = m < rows && k < a.k ? any_load(a.x, a.x_dtype, (m0 + m) * a.ldx + k) : 0.f;
+        if (a.activation == LVSA_W4_ACT_SILU) v[e] = v[e] / (1.f + expf(-v[e]));
+      }
+      for (int part = 0; part < p.parts; ++part) {
+        float sum = 0.f;
+        uint4 packed;
+        __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(&packed);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          h[e] = __float2bfloat16_rn(v[e]);
+          const float back = __bfloat162float(h[e]);
+          v[e] -= back;
+          sum += back;
+        }
+#pragma unroll
+        for (int w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if (m < rows) {
+          const int c = m * p.parts + part;
+          *reinterpret_cast<uint4*>(xs + static_cast<int64_t>(c) * p.pitch + 8 * o) = packed;
+          if (o % kLanes == 0) x_sums[o / kLanes * kCols + c] = -1.5f * sum;
+        }
+      }
+    }
+  };
+  // Columns that no row has are never written; their sums, and what the
+  // lanes of those columns hold, are zero.
+  for (int i = threadIdx.x; i < p.chunk_tiles * kBlocks * kCols; i += kThreadsW4)
+    if (i % kCols >= cols) x_sums[i] = 0.f;
+  const bool whole = p.chunk_tiles >= p.k_tiles;
+  if (whole) stage(0);
+  __syncthreads();
+
+  int slot = threadIdx.x;
+  for (int row_tile = blockIdx.x; row_tile < p.row_tiles; row_tile += gridDim.x) {
+    float acc[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
+    int tile = warp;
+    for (int first = 0; first < p.k_tiles; first += p.chunk_tiles) {
+      if (!whole) {
+        __syncthreads();
+        stage(first);
+        __syncthreads();
+      }
+      for (; tile < min(p.k_tiles, first + p.chunk_tiles); tile += kWarpsW4) {
+        copy_async_wait_but<kDepth - 1>();
+        const uint4 w = ring[slot];
+        const Word word = scale_ring[slot];
+        fetch();
+        slot += kThreadsW4;
+        if (slot >= kDepth * kThreadsW4) slot -= kDepth * kThreadsW4;
+        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        uint32_t scale_pairs[kBlocks];
+        if constexpr (HALVES) {
+          scale_pairs[0] = word.x;
+          scale_pairs[1] = word.y;
+        } else {
+          scale_pairs[0] = word;
+        }
+        uint4 b[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int c = 8 * t + r;  // this lane's column of x
+          const uint4* from = reinterpret_cast<const uint4*>(xs + static_cast<int64_t>(c) * p.pitch + (tile - first) * kTileK);
+          b[t][0] = c < cols ? from[j] : make_uint4(0u, 0u, 0u, 0u);
+          b[t][1] = c < cols ? from[4 + j] : make_uint4(0u, 0u, 0u, 0u);
+        }
+        float part[NT][4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          uint32_t f[4];
+          weights(words[s], f);
+          const bool start = s == 0 || (HALVES && s == 2), end = s == 3 || (HALVES && s == 1);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint4& q = b[t][s >> 1];
+            if (start) {
+              const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+              mma(part[t], f, s & 1 ? q.z : q.x, s & 1 ? q.w : q.y, zero);
+            } else {
+              mma(part[t], f, s & 1 ? q.z : q.x, s & 1 ? q.w : q.y, part[t]);
+            }
+            if (end) {
+              constexpr int kLast = kBlocks - 1;
+              const int h = HALVES ? s >> 1 : kLast;
+              const float2 off = *reinterpret_cast<const float2*>(x_sums + ((tile - first) * kBlocks + h) * kCols + 8 * t + 2 * j);
+              const TSc* sc = reinterpret_cast<const TSc*>(&scale_pairs[h]);
+              const float lo = to_f(sc[0]), hi = to_f(sc[1]);
+              acc[t][0] += lo * (part[t][0] + off.x);
+              acc[t][1] += lo * (part[t][1] + off.y);
+              acc[t][2] += hi * (part[t][2] + off.x);
+              acc[t][3] += hi * (part[t][3] + off.y);
+            }
+          }
+        }
+      }
+    }
+    // Join the warps' sums and the parts.
+    __syncthreads();  // the sums of the row of tiles before are read
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 8 * t + 2 * j + (i & 1);
+        if (c < cols) joined[(warp * kCols + c) * kTileN + r + 8 * (i >> 1)] = acc[t][i];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * kTileN; i += kThreadsW4) {
+      const int m = i / kTileN, row = i % kTileN;
+      const int64_t n = static_cast<int64_t>(row_tile) * kTileN + row;
+      float sum = 0.f;
+      for (int part = p.parts - 1; part >= 0; --part)  // the small parts first
+#pragma unroll
+        for (int w = 0; w < kWarpsW4; ++w) sum += joined[(w * kCols + m * p.parts + part) * kTileN + row];
+      sum *= 16.f;
+      if (n < a.n) {
+        if (a.bias) sum += any_load(a.bias, a.bias_dtype, n);
+        any_store(a.out, a.out_dtype, (m0 + m) * a.ldo + n, sum);
+      }
+    }
+  }
+  copy_async_wait_but<0>();
+}
+
+int shared_bytes(int nt, bool halves, int chunk_tiles, int cols, int pitch) {
+  return kDepth * kThreadsW4 * (16 + (halves ? 8 : 4)) + kWarpsW4 * 8 * nt * kTileN * 4 +
+         chunk_tiles * (halves ? 2 : 1) * 8 * nt * 4 + cols * pitch * 2;
+}
+// Columns of x lie 64 bytes beyond a multiple of 128 apart: the 8 x 4 lanes' 16 bytes fall on all banks.
+int column_pitch(int chunk_tiles) { return chunk_tiles * kTileK + 32; }
+
+template <int NT, bool HALVES, typename TSc>
+int launch(W4Params p, cudaStream_t s) {
+  const int sms = device_sms();
+  if (sms < 1) return LVSA_ERR_CUDA;
+  p.pass_rows = std::min(p.a.m, 8 * NT / p.parts);
+  const int cols = p.pass_rows * p.parts;
+  p.chunk_tiles = p.k_tiles;
+  while (shared_bytes(NT, HALVES, p.chunk_tiles, cols, column_pitch(p.chunk_tiles)) > kMaxShared)
+    p.chunk_tiles = (p.chunk_tiles / 2 + kWarpsW4 - 1) / kWarpsW4 * kWarpsW4;
+  p.pitch = column_pitch(p.chunk_tiles);
+  const int shared = shared_bytes(NT, HALVES, p.chunk_tiles, cols, p.pitch);
+  auto kern = w4_linear_kernel<NT, HALVES, TSc>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess) return LVSA_ERR_CUDA;
+  const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows;
+  const dim3 grid(std::min(p.row_tiles, std::max(1, sms / passes)), passes);
+  kern<<<grid, kThreadsW4, shared, s>>>(p);
+  return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
+}
+
+template <bool HALVES, typename TSc>
+int launch_columns(const W4Params& p, cudaStream_t s) {
+  const int64_t cols = static_cast<int64_t>(p.a.m) * p.parts;
+  if (cols <= 8) return launch<1, HALVES, TSc>(p, s);
+  return cols <= 16 ? launch<2, HALVES, TSc>(p, s) : launch<4, HALVES, TSc>(p, s);
+}
+
+}  // namespace
+}  // namespace lvsa
+
+extern "C" int lvsa_w4_bytes(int32_t n, int32_t k, int64_t* bytes) {
+  using namespace lvsa;
+  if (!bytes || n < 1 || k < 1) return LVSA_ERR_INVALID_ARG;
+  *bytes = (static_cast<int64_t>(n) + kTileN - 1) / kTileN * ((static_cast<int64_t>(k) + kTileK - 1) / kTileK) * 512;
+  return LVSA_OK;
+}
+
+extern "C" int lvsa_w4_pack(const int8_t* codes, int64_t ld, int32_t n, int32_t k, void* tiles, void* stream) {
+  using namespace lvsa;
+  int64_t bytes = 0;
+  const int st = lvsa_w4_bytes(n, k, &bytes);
+  if (st != LVSA_OK) return st;
+  if (!codes || !tiles || ld < k) return LVSA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(tiles) & 15) return LVSA_ERR_ALIGNMENT;
+  const int64_t total = bytes / 16, blocks = (total + 255) / 256;
+  if (blocks > INT32_MAX) return LVSA_ERR_UNSUPPORTED;
+  w4_pack_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      codes, ld, n, k, (k + kTileK - 1) / kTileK, total, static_cast<uint4*>(tiles));
+  return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
+}
+
+extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
+  using namespace lvsa;
+  if (!a || a->m < 0 || a->n < 1 || a->k < 1) return LVSA_ERR_INVALID_ARG;
+  if (a->group != 32 && a->group != 64 && a->group != 128) return LVSA_ERR_UNSUPPORTED;
+  if (!known_type(a->x_dtype) || !known_type(a->out_dtype) || (a->bias && !known_type(a->bias_dtype)) ||
+      (a->scale_dtype != LVSA_DTYPE_BF16 && a->scale_dtype != LVSA_DTYPE_F16) || a->n > INT32_MAX - kTileN ||
+      a->k > INT32_MAX - kTileK)
+    return LVSA_ERR_UNSUPPORTED;
+  if (a->activation != LVSA_W4_ACT_NONE && a->activation != LVSA_W4_ACT_SILU) return LVSA_ERR_INVALID_ARG;
+  if (!a->tiles || !a->scales || (a->m > 0 && (!a->x || !a->out || a->ldx < a->k || a->ldo < a->n))) return LVSA_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(a->tiles) & 15) || (reinterpret_cast<uintptr_t>(a->scales) & 7)) return LVSA_ERR_ALIGNMENT;
+  if (a->m == 0) return LVSA_OK;
+  W4Params p{};
+  p.a = *a;
+  p.k_tiles = (a->k + kTileK - 1) / kTileK;
+  p.row_tiles = (a->n + kTileN - 1) / kTileN;
+  p.parts = a->x_dtype == LVSA_DTYPE_F32 ? 3 : a->x_dtype == LVSA_DTYPE_F16 || a->activation != LVSA_W4_ACT_NONE ? 2 : 1;
+  if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a->scale_dtype == LVSA_DTYPE_BF16)
+    return a->group == 32 ? launch_columns<true, __nv_bfloat16>(p, s) : launch_columns<false, __nv_bfloat16>(p, s);
+  return a->group == 32 ? launch_columns<true, __half>(p, s) : launch_columns<false, __half>(p, s);
+}

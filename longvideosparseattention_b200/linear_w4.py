@@ -1,0 +1,138 @@
+"""Linear layers with 4-bit weights and a scale for each group of columns, for
+few rows: the Linears whose time is that of reading their weights.
+
+In a diffusion transformer these are the ones that the time embedding passes
+through, with one row a sequence or a latent frame: the shift, scale and gate
+vectors of every block (``block_norm``) come from a Linear of SiLU(embedding)
+whose weights are a large part of the model.  An addition of this package: the
+reference leaves them to the model.
+
+    w = quantize_w4(block.modulation.weight)               # once
+    shift, scale, gate = linear_w4(temb, w, bias, "silu").chunk(3, dim=-1)
+
+W[n, k] is approximated by scale[n, k // group] * code[n, k], codes -8 .. 7;
+``pack_w4`` takes codes and scales of another quantiser.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from .block_sparse import _stream_ptr
+
+_DT = {torch.bfloat16: N.LVSA_DTYPE_BF16, torch.float16: N.LVSA_DTYPE_F16, torch.float32: N.LVSA_DTYPE_F32}
+_ACT = {None: N.LVSA_W4_ACT_NONE, "silu": N.LVSA_W4_ACT_SILU}
+GROUPS = (32, 64, 128)
+
+
+@dataclass(frozen=True)
+class W4Weight:
+    """A [n, k] weight laid out for ``linear_w4`` (made by ``pack_w4``)."""
+
+    n: int
+    k: int
+    group: int
+    tiles: torch.Tensor   # uint8
+    scales: torch.Tensor  # bf16 / fp16
+
+    @property
+    def device(self) -> torch.device:
+        return self.tiles.device
+
+
+def pack_w4(codes: torch.Tensor, scales: torch.Tensor, group: int) -> W4Weight:
+    """Lay out codes [n, k] (int8, -8 .. 7) with scales [n, ceil(k / group)]
+    (bf16 / fp16; group 32, 64 or 128).  Codes out of range are not looked
+    for: their low four bits count."""
+    if not codes.is_cuda:
+        raise RuntimeError("pack_w4 needs CUDA tensors (no CPU fallback)")
+    if codes.dtype != torch.int8 or scales.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"pack_w4: int8 codes and bf16 / fp16 scales expected, got {codes.dtype} and {scales.dtype}")
+    if group not in GROUPS:
+        raise ValueError(f"pack_w4: group must be one of {GROUPS}, got {group}")
+    if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] < 1:
+        raise ValueError(f"pack_w4: codes must be [n, k], got {tuple(codes.shape)}")
+    n, k = codes.shape
+    if scales.device != codes.device or tuple(scales.shape) != (n, -(-k // group)):
+        raise ValueError(f"pack_w4: scales must be [{n}, {-(-k // group)}] on {codes.device}, got "
+                         f"{tuple(scales.shape)} on {scales.device}")
+    codes = codes if codes.stride(1) == 1 and codes.stride(0) >= k else codes.contiguous()
+    lib, size = N.load(), ctypes.c_int64()
+    N.check(lib.lvsa_w4_bytes(n, k, ctypes.byref(size)), "lvsa_w4_bytes")
+    tiles = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
+    with torch.cuda.device(codes.device):
+        st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0), n, k, tiles.data_ptr(), _stream_ptr(codes.device))
+    N.check(st, "lvsa_w4_pack")
+    rows, blocks = -(-n // 16), -(-k // group)
+    if group == 32:
+        blocks = -(-k // 64) * 2
+    s = torch.nn.functional.pad(scales.detach(), (0, blocks - scales.shape[1], 0, rows * 16 - n)).view(rows, 2, 8, blocks)
+    if group == 32:  # [row of tiles, k tile, row, half, row or row + 8]
+        s = s.unflatten(3, (-1, 2)).permute(0, 3, 2, 4, 1)
+    else:            # [row of tiles, group, row, row or row + 8]
+        s = s.permute(0, 3, 2, 1)
+    return W4Weight(n, k, group, tiles, s.contiguous())
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 64, scale_dtype: torch.dtype = torch.bfloat16) -> W4Weight:
+    """Round a weight [n, k] to the nearest code -7 .. 7 of its group's scale,
+    the largest size in the group over 7."""
+    if weight.dim() != 2:
+        raise ValueError(f"quantize_w4: weight must be [n, k], got {tuple(weight.shape)}")
+    if group not in GROUPS:
+        raise ValueError(f"quantize_w4: group must be one of {GROUPS}, got {group}")
+    if scale_dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"quantize_w4: scale_dtype must be bf16 or fp16, got {scale_dtype}")
+    n, k = weight.shape
+    w = torch.nn.functional.pad(weight.detach().float(), (0, -k % group)).unflatten(1, (-1, group))
+    scales = (w.abs().amax(-1) / 7).to(scale_dtype)
+    step = scales.float()[..., None]
+    codes = torch.where(step > 0, w / step, 0.0).round_().clamp_(-7, 7).to(torch.int8).flatten(1)[:, :k]
+    return pack_w4(codes, scales, group)
+
+
+def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None,
+              activation: Optional[str] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x) W^T + bias: x [..., k] -> [..., n] in ``out_dtype`` (default x's).
+
+    x, bias and output in bf16, fp16 or fp32; ``activation`` None or "silu",
+    in fp32.  Products are exact and sums fp32, with one rounding of the
+    result.  Made for few rows (a row a sequence or a latent frame); each
+    further 32 / 16 / 10 rows (bf16 / fp16 or with an activation / fp32) read
+    the weights once more.  Inference only: x must not require grad."""
+    if not x.is_cuda:
+        raise RuntimeError("linear_w4 needs CUDA tensors (no CPU fallback)")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if x.dtype not in _DT or out_dtype not in _DT or (bias is not None and bias.dtype not in _DT):
+        raise TypeError("linear_w4: x, bias and output in bf16, fp16 or fp32")
+    if activation not in _ACT:
+        raise ValueError(f"linear_w4: activation must be None or 'silu', got {activation!r}")
+    if x.dim() < 1 or x.shape[-1] != weight.k:
+        raise ValueError(f"linear_w4: features of x {tuple(x.shape)} do not match weight [{weight.n}, {weight.k}]")
+    if weight.device != x.device or (bias is not None and bias.device != x.device):
+        raise ValueError("linear_w4: x, weight and bias must be on one device")
+    if bias is not None and tuple(bias.shape) != (weight.n,):
+        raise ValueError(f"linear_w4: bias must be [{weight.n}], got {tuple(bias.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad() or on detached tensors")
+    rows = x if x.dim() == 2 else x.reshape(-1, weight.k)
+    if rows.stride(1) != 1 or rows.stride(0) < weight.k:
+        rows = rows.contiguous()
+    if bias is not None and bias.stride(0) != 1:
+        bias = bias.contiguous()
+    m = rows.shape[0]
+    out = torch.empty(m, weight.n, dtype=out_dtype, device=x.device)
+    if m:
+        args = N.LvsaW4Linear(rows.data_ptr(), weight.tiles.data_ptr(), weight.scales.data_ptr(),
+                              bias.data_ptr() if bias is not None else None, out.data_ptr(), rows.stride(0), weight.n,
+                              m, weight.n, weight.k, weight.group, _DT[x.dtype], _DT[out_dtype],
+                              _DT[bias.dtype] if bias is not None else 0, _DT[weight.scales.dtype], _ACT[activation])
+        with torch.cuda.device(x.device):
+            st = N.load().lvsa_w4_linear(ctypes.byref(args), _stream_ptr(x.device))
+        N.check(st, "lvsa_w4_linear")
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.n)

@@ -1,0 +1,68 @@
+"""Linear with 4-bit weights, host side: the C ABI's structure and argument
+checks (no launch), and the refusal of CPU tensors."""
+
+import ctypes
+import os
+import subprocess
+import tempfile
+
+import pytest
+import torch
+
+from longvideosparseattention_b200 import _native as N
+from tests.conftest import ROOT
+
+FAKE = 1 << 20  # aligned, never read
+
+
+def _args(**kw):
+    a = N.LvsaW4Linear(FAKE, FAKE, FAKE, None, FAKE, 64, 32, 0, 32, 64, 64, 0, 0, 0, 0, 0)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_struct_layout():
+    probe = r'''
+#include <stdio.h>
+#include <stddef.h>
+#include "lvsa_b200.h"
+int main(void){ printf("%zu %zu %zu\n", sizeof(LvsaW4Linear), offsetof(LvsaW4Linear, m), offsetof(LvsaW4Linear, activation)); return 0;}
+'''
+    with tempfile.TemporaryDirectory() as d:
+        c, exe = os.path.join(d, "p.c"), os.path.join(d, "p")
+        with open(c, "w") as fh:
+            fh.write(probe)
+        subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), c, "-o", exe], check=True)
+        got = [int(v) for v in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(N.LvsaW4Linear), N.LvsaW4Linear.m.offset, N.LvsaW4Linear.activation.offset]
+
+
+def test_checks():
+    lib = N.load()
+    call = lambda a: lib.lvsa_w4_linear(ctypes.byref(a), None)  # noqa: E731
+    assert call(_args()) == N.LVSA_OK  # no rows: nothing to launch
+    assert lib.lvsa_w4_linear(None, None) == N.LVSA_ERR_INVALID_ARG
+    for bad in (dict(m=-1), dict(n=0), dict(k=0), dict(tiles=None), dict(scales=None), dict(activation=2),
+                dict(m=1, x=None), dict(m=1, out=None), dict(m=1, ldx=63), dict(m=1, ldo=31)):
+        assert call(_args(**bad)) == N.LVSA_ERR_INVALID_ARG, bad
+    for bad in (dict(group=16), dict(group=256), dict(x_dtype=2), dict(out_dtype=9), dict(bias=FAKE, bias_dtype=2),
+                dict(scale_dtype=3)):
+        assert call(_args(**bad)) == N.LVSA_ERR_UNSUPPORTED, bad
+    for bad in (dict(tiles=FAKE + 8), dict(scales=FAKE + 4)):
+        assert call(_args(**bad)) == N.LVSA_ERR_ALIGNMENT, bad
+    size = ctypes.c_int64()
+    assert lib.lvsa_w4_bytes(17, 65, ctypes.byref(size)) == N.LVSA_OK and size.value == 2 * 2 * 512
+    assert lib.lvsa_w4_bytes(0, 65, ctypes.byref(size)) == N.LVSA_ERR_INVALID_ARG
+    assert lib.lvsa_w4_bytes(1, 1, None) == N.LVSA_ERR_INVALID_ARG
+    assert lib.lvsa_w4_pack(None, 1, 1, 1, FAKE, None) == N.LVSA_ERR_INVALID_ARG
+    assert lib.lvsa_w4_pack(FAKE, 7, 1, 8, FAKE, None) == N.LVSA_ERR_INVALID_ARG
+    assert lib.lvsa_w4_pack(FAKE, 8, 1, 8, FAKE + 8, None) == N.LVSA_ERR_ALIGNMENT
+
+
+def test_cpu_tensors_are_refused():
+    from longvideosparseattention_b200.linear_w4 import pack_w4, quantize_w4
+    with pytest.raises(RuntimeError):
+        pack_w4(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.bfloat16), 64)
+    with pytest.raises(RuntimeError):
+        quantize_w4(torch.zeros(4, 64))
