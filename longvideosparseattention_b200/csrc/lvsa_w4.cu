@@ -15,11 +15,11 @@
 // two for f16 and for an activation of a 16-bit x (16 bits), three for fp32
 // (24 bits).  With few rows the columns they take are free.
 //
-// Work.  A CTA an SM, 16 warps; a CTA takes rows of tiles (16 rows of
-// weights) in turn and its warps share a row's tiles of 64 columns, so that
-// even a narrow Linear keeps every SM reading.  Tiles come through a ring in
-// shared memory (cp.async, a thread's own 16 bytes: no barrier), which runs
-// on across rows of tiles while the warps' sums are joined.
+// Work.  A CTA an SM, 16 warps; x, as parts, in its shared memory.  A warp
+// takes a row of tiles (16 rows of weights), or one of `splits` stretches of
+// its columns where there are few rows, and streams its tiles through
+// registers, kAhead of them on their way.  Stretches are joined through
+// shared memory in order.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -34,14 +34,18 @@ namespace {
 
 constexpr int kTileN = 16, kTileK = 64;
 constexpr int kWarpsW4 = 16, kThreadsW4 = 32 * kWarpsW4;
-constexpr int kDepth = 8;                      // tiles of a warp on their way
+constexpr int kAhead = 8;                      // tiles of a warp on their way
 constexpr int kMaxShared = 227 * 1024 - 1024;
 
 struct W4Params {
   LvsaW4Linear a;
-  int32_t k_tiles, row_tiles, parts, pass_rows;  // rows of x a pass (blockIdx.y)
-  int32_t chunk_tiles;                           // k tiles of x held at once
-  int32_t pitch;                                 // bf16 values between the columns of x held
+  int32_t k_tiles, row_tiles, parts;
+  int32_t pass_rows;      // rows of x a pass (blockIdx.y)
+  int32_t splits, slots;  // stretches of a row of tiles; rows of tiles of a CTA at once
+  int32_t stretch;        // k tiles of a stretch
+  int32_t chunk;          // k tiles of each stretch for which x is held at once
+  int32_t pitch;          // bf16 values between the columns of x held
+  int32_t x_vectors;      // x may be read 8 values at a time
 };
 
 // ---- layout: lane l = 4 r + j of a tile holds rows r and r + 8, columns
@@ -79,72 +83,63 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// The A fragment of a word: 1 + u / 16 as bf16 pairs.
+// The A fragment of a word: 1 + u / 16 as bf16 pairs, or q / 16.
+template <bool CENTRED>
 __device__ __forceinline__ void weights(uint32_t w, uint32_t (&a)[4]) {
   constexpr uint32_t kMask = 0x00780078u, kOne = 0x3f803f80u;
   a[0] = (w & kMask) | kOne;
   a[1] = ((w >> 4) & kMask) | kOne;
   a[2] = ((w >> 8) & kMask) | kOne;
   a[3] = (__funnelshift_r(w, w, 12) & kMask) | kOne;
+  if constexpr (CENTRED) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __nv_bfloat162& h = reinterpret_cast<__nv_bfloat162&>(a[i]);
+      h = __hsub2(h, __floats2bfloat162_rn(1.5f, 1.5f));
+    }
+  }
 }
 
-template <int N>
-__device__ __forceinline__ void copy_async_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns.
-template <int NT, bool HALVES, typename TSc>
+// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns;
+// CENTRED: codes as q / 16 themselves rather than 1.5 + q / 16.
+template <int NT, bool HALVES, bool CENTRED, typename TSc>
 __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
   using Word = typename std::conditional<HALVES, uint2, uint32_t>::type;
   constexpr int kBlocks = HALVES ? 2 : 1;  // sums of x a k tile
   constexpr int kCols = 8 * NT;
   extern __shared__ uint4 shared_w4[];
-  uint4* const ring = shared_w4;                                                   // [depth][threads]
-  Word* const scale_ring = reinterpret_cast<Word*>(ring + kDepth * kThreadsW4);    // [depth][threads]
-  float* const joined = reinterpret_cast<float*>(scale_ring + kDepth * kThreadsW4);  // [warp][column][row]
-  float* const x_sums = joined + kWarpsW4 * kCols * kTileN;                        // [block][column]
-  __nv_bfloat16* const xs = reinterpret_cast<__nv_bfloat16*>(x_sums + p.chunk_tiles * kBlocks * kCols);  // [column][pitch]
+  __nv_bfloat16* const xs = reinterpret_cast<__nv_bfloat16*>(shared_w4);  // [column][pitch]
 
   const LvsaW4Linear& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
   const int m0 = blockIdx.y * p.pass_rows, rows = min(p.pass_rows, a.m - m0), cols = rows * p.parts;
-
-  // This warp's tiles: warp, warp + 16, ... of every row of tiles that is the CTA's.
+  float* const x_sums = reinterpret_cast<float*>(xs + static_cast<int64_t>(p.pass_rows) * p.parts * p.pitch);  // [block][column]
+  float* const joined = x_sums + (CENTRED ? 0 : p.splits * p.chunk * kBlocks * kCols);                        // [warp][column][row]
+  const int split = warp / p.slots, slot = warp - split * p.slots;  // warps beyond splits x slots have nothing
+  const int k_first = split * p.stretch, k_last = split < p.splits ? min(p.k_tiles, k_first + p.stretch) : k_first;
   const int scale_words = HALVES ? p.k_tiles : (a.k + a.group - 1) / a.group;  // of a row of tiles, times 8
   const int scale_shift = a.group == 128 ? 1 : 0;
-  int fetch_row = blockIdx.x, fetch_tile = warp, fetch_slot = threadIdx.x;
-  auto fetch = [&]() {
-    if (fetch_row < p.row_tiles && fetch_tile < p.k_tiles) {
-      const int64_t tile = static_cast<int64_t>(fetch_row) * p.k_tiles + fetch_tile;
-      copy_async<16>(ring + fetch_slot, static_cast<const uint4*>(a.tiles) + tile * 32 + lane);
-      copy_async<sizeof(Word)>(scale_ring + fetch_slot,
-                               static_cast<const Word*>(a.scales) +
-                                   (static_cast<int64_t>(fetch_row) * scale_words + (fetch_tile >> scale_shift)) * 8 + r);
-      fetch_slot += kThreadsW4;
-      if (fetch_slot >= kDepth * kThreadsW4) fetch_slot -= kDepth * kThreadsW4;
-      fetch_tile += kWarpsW4;
-      if (fetch_tile >= p.k_tiles) {
-        fetch_tile = warp;
-        fetch_row += gridDim.x;
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < kDepth; ++i) fetch();
 
-  // x's columns from k tile `first` on, as bf16 parts, and -1.5 times their
-  // sums: a thread takes 8 values, the threads of a block of columns add up.
+  // x's columns of chunk `first` of every stretch, as bf16 parts, and -1.5
+  // times their sums: a thread takes 8 values, the threads of a block add up.
   auto stage = [&](int first) {
-    const int tiles = min(p.chunk_tiles, p.k_tiles - first), octets = tiles * (kTileK / 8);
+    const int held = p.splits * p.chunk, octets = held * (kTileK / 8);
     constexpr int kLanes = HALVES ? 4 : 8;  // threads a block
     for (int i = threadIdx.x; i < (rows * octets + 31) / 32 * 32; i += kThreadsW4) {
       const int m = i / octets, o = i - m * octets;  // octets is a multiple of 8: a block lies in one row
+      const int at = o / 8, stretch = at / p.chunk, tile = first + at - stretch * p.chunk;
+      const int64_t k0 = static_cast<int64_t>(stretch * p.stretch + tile) * kTileK + o % 8 * 8;
+      const int64_t end = tile < p.stretch && m < rows ? a.k : 0;  // past a stretch's end: zeros, not used
       float v[8];
+      if (p.x_vectors && k0 + 8 <= end) {
+        any_load<8>(a.x, a.x_dtype, (m0 + m) * a.ldx + k0, v);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t k = static_cast<int64_t>(first) * kTileK + 8 * o + e;
-        v[e] = m < rows && k < a.k ? any_load(a.x, a.x_dtype, (m0 + m) * a.ldx + k) : 0.f;
-        if (a.activation == LVSA_W4_ACT_SILU) v[e] = v[e] / (1.f + expf(-v[e]));
+        for (int e = 0; e < 8; ++e) v[e] = k0 + e < end ? any_load(a.x, a.x_dtype, (m0 + m) * a.ldx + k0 + e) : 0.f;
+      }
+      if (a.activation == LVSA_W4_ACT_SILU) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + expf(-v[e]));
       }
       for (int part = 0; part < p.parts; ++part) {
         float sum = 0.f;
@@ -157,46 +152,72 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
           v[e] -= back;
           sum += back;
         }
+        const int c = m * p.parts + part;
+        if (m < rows) *reinterpret_cast<uint4*>(xs + c * p.pitch + 8 * o) = packed;
+        if constexpr (!CENTRED) {
 #pragma unroll
-        for (int w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        if (m < rows) {
-          const int c = m * p.parts + part;
-          *reinterpret_cast<uint4*>(xs + static_cast<int64_t>(c) * p.pitch + 8 * o) = packed;
-          if (o % kLanes == 0) x_sums[o / kLanes * kCols + c] = -1.5f * sum;
+          for (int w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+          if (m < rows && o % kLanes == 0) x_sums[o / kLanes * kCols + c] = -1.5f * sum;
         }
       }
     }
   };
-  // Columns that no row has are never written; their sums, and what the
-  // lanes of those columns hold, are zero.
-  for (int i = threadIdx.x; i < p.chunk_tiles * kBlocks * kCols; i += kThreadsW4)
-    if (i % kCols >= cols) x_sums[i] = 0.f;
-  const bool whole = p.chunk_tiles >= p.k_tiles;
-  if (whole) stage(0);
-  __syncthreads();
 
-  int slot = threadIdx.x;
-  for (int row_tile = blockIdx.x; row_tile < p.row_tiles; row_tile += gridDim.x) {
+  // This lane's columns as indices of 16 bytes (known to be shared memory, as
+  // pointers kept in an array are not).  Columns past the last are sums of
+  // another column's x, and not used.
+  int x_lane[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int c = 8 * t + r;
+    x_lane[t] = ((c < cols ? c : 0) * p.pitch + split * p.chunk * kTileK) / 8 + j;
+  }
+  const int sums_lane = split * p.chunk * kBlocks * kCols + 2 * j;
+
+  const bool whole = p.chunk >= p.stretch;
+  const int turns = (p.row_tiles + gridDim.x * p.slots - 1) / (gridDim.x * p.slots);
+  for (int turn = 0; turn < turns; ++turn) {
+    // Neighbouring CTAs take neighbouring rows of tiles: the SMs' shares differ by one at most.
+    const int row_tile = (turn * p.slots + slot) * gridDim.x + blockIdx.x;
+    const int last = row_tile < p.row_tiles ? k_last : k_first;
+    const uint4* tiles = static_cast<const uint4*>(a.tiles) + static_cast<int64_t>(row_tile) * p.k_tiles * 32 + lane;
+    const Word* scales = static_cast<const Word*>(a.scales) + static_cast<int64_t>(row_tile) * scale_words * 8 + r;
+    uint4 w[kAhead];
+    Word sc[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (k_first + u < last) {
+        w[u] = __ldg(tiles + (k_first + u) * 32);
+        sc[u] = __ldg(scales + ((k_first + u) >> scale_shift) * 8);
+      }
     float acc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[t][i] = 0.f;
-    int tile = warp;
-    for (int first = 0; first < p.k_tiles; first += p.chunk_tiles) {
-      if (!whole) {
-        __syncthreads();
+
+    for (int first = 0; first < p.stretch; first += p.chunk) {
+      if (!whole || turn == 0) {
+        if (turn + first > 0) __syncthreads();
         stage(first);
         __syncthreads();
       }
-      for (; tile < min(p.k_tiles, first + p.chunk_tiles); tile += kWarpsW4) {
-        copy_async_wait_but<kDepth - 1>();
-        const uint4 w = ring[slot];
-        const Word word = scale_ring[slot];
-        fetch();
-        slot += kThreadsW4;
-        if (slot >= kDepth * kThreadsW4) slot -= kDepth * kThreadsW4;
-        const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+      const int end = min(last, k_first + first + p.chunk);
+      // One tile from w[u], in whose place the one kAhead later is asked for.
+      auto tile_of = [&](int tile, int u, bool more) {
+        const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+        const Word word = sc[u];
+        if (more) {
+          w[u] = __ldg(tiles + (tile + kAhead) * 32);
+          sc[u] = __ldg(scales + ((tile + kAhead) >> scale_shift) * 8);
+        }
+        const int local = tile - k_first - first;
+        uint4 b[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          b[t][0] = shared_w4[x_lane[t] + local * (kTileK / 8)];
+          b[t][1] = shared_w4[x_lane[t] + local * (kTileK / 8) + 4];
+        }
         uint32_t scale_pairs[kBlocks];
         if constexpr (HALVES) {
           scale_pairs[0] = word.x;
@@ -204,20 +225,12 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
         } else {
           scale_pairs[0] = word;
         }
-        uint4 b[NT][2];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int c = 8 * t + r;  // this lane's column of x
-          const uint4* from = reinterpret_cast<const uint4*>(xs + static_cast<int64_t>(c) * p.pitch + (tile - first) * kTileK);
-          b[t][0] = c < cols ? from[j] : make_uint4(0u, 0u, 0u, 0u);
-          b[t][1] = c < cols ? from[4 + j] : make_uint4(0u, 0u, 0u, 0u);
-        }
         float part[NT][4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           uint32_t f[4];
-          weights(words[s], f);
-          const bool start = s == 0 || (HALVES && s == 2), end = s == 3 || (HALVES && s == 1);
+          weights<CENTRED>(words[s], f);
+          const bool start = s == 0 || (HALVES && s == 2), stop = s == 3 || (HALVES && s == 1);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             const uint4& q = b[t][s >> 1];
@@ -227,12 +240,12 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
             } else {
               mma(part[t], f, s & 1 ? q.z : q.x, s & 1 ? q.w : q.y, part[t]);
             }
-            if (end) {
-              constexpr int kLast = kBlocks - 1;
-              const int h = HALVES ? s >> 1 : kLast;
-              const float2 off = *reinterpret_cast<const float2*>(x_sums + ((tile - first) * kBlocks + h) * kCols + 8 * t + 2 * j);
-              const TSc* sc = reinterpret_cast<const TSc*>(&scale_pairs[h]);
-              const float lo = to_f(sc[0]), hi = to_f(sc[1]);
+            if (stop) {
+              const int h = HALVES ? s >> 1 : 0;
+              float2 off = make_float2(0.f, 0.f);
+              if constexpr (!CENTRED) off = *reinterpret_cast<const float2*>(x_sums + sums_lane + (local * kBlocks + h) * kCols + 8 * t);
+              const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[h]);
+              const float lo = to_f(pair[0]), hi = to_f(pair[1]);
               acc[t][0] += lo * (part[t][0] + off.x);
               acc[t][1] += lo * (part[t][1] + off.y);
               acc[t][2] += hi * (part[t][2] + off.x);
@@ -240,66 +253,95 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
             }
           }
         }
+      };
+      int base = k_first + first;
+      for (; base + 2 * kAhead <= last && base + kAhead <= end; base += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) tile_of(base + u, u, true);
+      }
+      for (; base < end; base += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+          if (base + u < end) tile_of(base + u, u, base + u + kAhead < last);
       }
     }
-    // Join the warps' sums and the parts.
-    __syncthreads();  // the sums of the row of tiles before are read
+    // Join the stretches and the parts: [row of tiles of the CTA][split][column][row].
+    if (turn > 0) __syncthreads();  // the turn before has been read
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = 8 * t + 2 * j + (i & 1);
-        if (c < cols) joined[(warp * kCols + c) * kTileN + r + 8 * (i >> 1)] = acc[t][i];
+        if (c < cols && split < p.splits) joined[((slot * p.splits + split) * kCols + c) * kTileN + r + 8 * (i >> 1)] = acc[t][i];
       }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * kTileN; i += kThreadsW4) {
-      const int m = i / kTileN, row = i % kTileN;
-      const int64_t n = static_cast<int64_t>(row_tile) * kTileN + row;
+    for (int i = threadIdx.x; i < p.slots * rows * kTileN; i += kThreadsW4) {
+      const int row = i % kTileN, m = i / kTileN % rows, which = i / (kTileN * rows);
+      const int64_t n = static_cast<int64_t>((turn * p.slots + which) * gridDim.x + blockIdx.x) * kTileN + row;
+      if (n >= a.n) continue;
       float sum = 0.f;
       for (int part = p.parts - 1; part >= 0; --part)  // the small parts first
-#pragma unroll
-        for (int w = 0; w < kWarpsW4; ++w) sum += joined[(w * kCols + m * p.parts + part) * kTileN + row];
+        for (int s = 0; s < p.splits; ++s)
+          sum += joined[((which * p.splits + s) * kCols + m * p.parts + part) * kTileN + row];
       sum *= 16.f;
-      if (n < a.n) {
-        if (a.bias) sum += any_load(a.bias, a.bias_dtype, n);
-        any_store(a.out, a.out_dtype, (m0 + m) * a.ldo + n, sum);
-      }
+      if (a.bias) sum += any_load(a.bias, a.bias_dtype, n);
+      any_store(a.out, a.out_dtype, (m0 + m) * a.ldo + n, sum);
     }
   }
-  copy_async_wait_but<0>();
 }
 
-int shared_bytes(int nt, bool halves, int chunk_tiles, int cols, int pitch) {
-  return kDepth * kThreadsW4 * (16 + (halves ? 8 : 4)) + kWarpsW4 * 8 * nt * kTileN * 4 +
-         chunk_tiles * (halves ? 2 : 1) * 8 * nt * 4 + cols * pitch * 2;
-}
 // Columns of x lie 64 bytes beyond a multiple of 128 apart: the 8 x 4 lanes' 16 bytes fall on all banks.
-int column_pitch(int chunk_tiles) { return chunk_tiles * kTileK + 32; }
+int column_pitch(int tiles) { return tiles * kTileK + 32; }
+int shared_bytes(int nt, bool halves, bool centred, int splits, int slots, int chunk, int cols) {
+  return cols * column_pitch(splits * chunk) * 2 + (centred ? 0 : splits * chunk * (halves ? 2 : 1) * 8 * nt * 4) +
+         splits * slots * 8 * nt * kTileN * 4;
+}
 
-template <int NT, bool HALVES, typename TSc>
+template <int NT, bool HALVES, bool CENTRED, typename TSc>
 int launch(W4Params p, cudaStream_t s) {
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
   p.pass_rows = std::min(p.a.m, 8 * NT / p.parts);
+  const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows, ctas = std::max(1, sms / passes);
+  // Rows of tiles of an SM; where they are fewer than the warps, more warps share one.
+  const int share = (p.row_tiles + ctas - 1) / ctas;
+  p.splits = 1;
+  while (2 * p.splits * share <= kWarpsW4 && 2 * p.splits <= p.k_tiles) p.splits *= 2;
   const int cols = p.pass_rows * p.parts;
-  p.chunk_tiles = p.k_tiles;
-  while (shared_bytes(NT, HALVES, p.chunk_tiles, cols, column_pitch(p.chunk_tiles)) > kMaxShared)
-    p.chunk_tiles = (p.chunk_tiles / 2 + kWarpsW4 - 1) / kWarpsW4 * kWarpsW4;
-  p.pitch = column_pitch(p.chunk_tiles);
-  const int shared = shared_bytes(NT, HALVES, p.chunk_tiles, cols, p.pitch);
-  auto kern = w4_linear_kernel<NT, HALVES, TSc>;
+  auto shared_of = [&]() { return shared_bytes(NT, HALVES, CENTRED, p.splits, p.slots, p.chunk, cols); };
+  for (;; p.splits /= 2) {
+    p.slots = std::min(share, kWarpsW4 / p.splits);
+    p.stretch = (p.k_tiles + p.splits - 1) / p.splits;
+    // All of x at once where it fits, else a multiple of kAhead tiles of each
+    // stretch, which are fewer and longer where even that does not.
+    p.chunk = p.stretch;
+    if (shared_of() > kMaxShared) {
+      p.chunk = p.chunk / kAhead * kAhead;
+      while (p.chunk > kAhead && shared_of() > kMaxShared) p.chunk -= kAhead;
+    }
+    if (p.chunk > 0 && shared_of() <= kMaxShared) break;
+    if (p.splits == 1) return LVSA_ERR_UNSUPPORTED;
+  }
+  p.pitch = column_pitch(p.splits * p.chunk);
+  auto kern = w4_linear_kernel<NT, HALVES, CENTRED, TSc>;
+  const int shared = shared_of();
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess) return LVSA_ERR_CUDA;
-  const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows;
-  const dim3 grid(std::min(p.row_tiles, std::max(1, sms / passes)), passes);
-  kern<<<grid, kThreadsW4, shared, s>>>(p);
+  kern<<<dim3(std::min(p.row_tiles, ctas), passes), kThreadsW4, shared, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-template <bool HALVES, typename TSc>
+template <bool HALVES, bool CENTRED, typename TSc>
 int launch_columns(const W4Params& p, cudaStream_t s) {
   const int64_t cols = static_cast<int64_t>(p.a.m) * p.parts;
-  if (cols <= 8) return launch<1, HALVES, TSc>(p, s);
-  return cols <= 16 ? launch<2, HALVES, TSc>(p, s) : launch<4, HALVES, TSc>(p, s);
+  if (cols <= 8) return launch<1, HALVES, CENTRED, TSc>(p, s);
+  return cols <= 16 ? launch<2, HALVES, CENTRED, TSc>(p, s) : launch<4, HALVES, CENTRED, TSc>(p, s);
+}
+
+template <typename TSc>
+int launch_form(const W4Params& p, cudaStream_t s) {
+  const bool centred = p.a.x_dtype == LVSA_DTYPE_F32 || p.a.out_dtype == LVSA_DTYPE_F32;
+  if (p.a.group == 32) return centred ? launch_columns<true, true, TSc>(p, s) : launch_columns<true, false, TSc>(p, s);
+  return centred ? launch_columns<false, true, TSc>(p, s) : launch_columns<false, false, TSc>(p, s);
 }
 
 }  // namespace
@@ -343,9 +385,8 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   p.k_tiles = (a->k + kTileK - 1) / kTileK;
   p.row_tiles = (a->n + kTileN - 1) / kTileN;
   p.parts = a->x_dtype == LVSA_DTYPE_F32 ? 3 : a->x_dtype == LVSA_DTYPE_F16 || a->activation != LVSA_W4_ACT_NONE ? 2 : 1;
+  p.x_vectors = vector_vector(Vector{a->x, a->ldx, 0, a->x_dtype}, 8);
   if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a->scale_dtype == LVSA_DTYPE_BF16)
-    return a->group == 32 ? launch_columns<true, __nv_bfloat16>(p, s) : launch_columns<false, __nv_bfloat16>(p, s);
-  return a->group == 32 ? launch_columns<true, __half>(p, s) : launch_columns<false, __half>(p, s);
+  return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_form<__nv_bfloat16>(p, s) : launch_form<__half>(p, s);
 }
