@@ -375,9 +375,10 @@ int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
  * r and r + 8 of a tile), [ceil(n / 16)][ceil(k / group)][8] words for group 64
  * or 128 and [ceil(n / 16)][T][8][2] words for group 32, 0 past the end.
  *
- * Products are exact (x as one to three bf16 parts, their number by what act
- * and x's type need) and sums fp32; one rounding to the output's type.  A row
- * of x that holds an infinity or NaN gives NaN. */
+ * Products are exact and sums fp32, with one rounding to the output's type; x
+ * enters as f16 parts of 64 (32) values over their power of two, 11 bits where
+ * x has no more or the output is bf16, else 22.  A row of x that holds an
+ * infinity or NaN gives infinities or NaN. */
 enum { LVSA_W4_ACT_NONE = 0, LVSA_W4_ACT_SILU = 1 };
 typedef struct LvsaW4Linear {
   const void* x;     /* [m, k], row stride ldx elements, bf16 / f16 / fp32       */

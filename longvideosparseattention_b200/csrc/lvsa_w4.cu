@@ -2,18 +2,18 @@
 // rows of x: out[m, n] = sum_k act(x[m, k]) s[n, k / group] q[n, k] (+ bias).
 // Bound: HBM, n k / 2 bytes of codes and 2 n k / group of scales read once.
 //
-// Arithmetic.  A code q = -8 .. 7 is stored as u = q + 8, and the bf16 number
-// with u in the top of its mantissa is w = 1 + u / 16, made from u by a shift
-// and one three-input operation for two codes; q = 16 (w - 1.5).  So with
-// x's bf16 parts as the other operand of m16n8k16 (weights as its 16 rows,
-// parts of rows of x as its 8 columns; bf16 products are exact, sums fp32)
-//   sum of a group = 16 (sum_k x w - 1.5 sum_k x),
-// where the second sum belongs to x and the 16 waits until the end.  The
-// offset costs two to three bits of the fp32 sum (w is 1.5 where q / 16 is
-// 0.3 on average), a subtraction a code would cost a third of the issue slots.
-// x enters as bf16 parts: one where it is bf16 and no activation applies,
-// two for f16 and for an activation of a 16-bit x (16 bits), three for fp32
-// (24 bits).  With few rows the columns they take are free.
+// Arithmetic.  A code q = -8 .. 7 is stored as u = q + 8.  Set into an f16
+// number's mantissa at its top, u makes 1 + u / 16, four bits lower 1 + u / 256;
+// one half-precision operation takes either to q / 16, exactly, so that two
+// codes cost 1.25 integer operations (the pipe that bounds this kernel next to
+// HBM) and one on the other pipe.  m16n8k16 multiplies (weights as its 16 rows,
+// parts of rows of x as its 8 columns; f16 products are exact, sums fp32).
+// x enters as f16 parts, one or two (11 or 22 bits), of x / 2^e, with e of the
+// largest of the 64 (32) values that one scale of the weights goes with: 2^e
+// joins that scale in fp32, and any x fits f16's range.  One part where that is
+// exact (a 16-bit x without an activation) or where the result is bf16 (2^-12
+// of x under 2^-9 of the result), two otherwise; with few rows the columns
+// are free.
 //
 // Work.  A CTA an SM, 16 warps; x, as parts, in its shared memory.  A warp
 // takes a row of tiles (16 rows of weights), or one of `splits` stretches of
@@ -33,9 +33,13 @@ namespace lvsa {
 namespace {
 
 constexpr int kTileN = 16, kTileK = 64;
-constexpr int kWarpsW4 = 16, kThreadsW4 = 32 * kWarpsW4;
-constexpr int kAhead = 8;                      // tiles of a warp on their way
 constexpr int kMaxShared = 227 * 1024 - 1024;
+// Warps of a CTA, and tiles of a warp on their way: as many warps as the
+// registers allow, 32 with one tile of columns.
+template <int NT>
+constexpr int kWarpsW4 = NT == 1 ? 32 : 16;
+template <int NT>
+constexpr int kAhead = NT == 1 ? 4 : 8;
 
 struct W4Params {
   LvsaW4Linear a;
@@ -52,7 +56,7 @@ struct W4Params {
 // 8 j .. 8 j + 7 and 32 + 8 j .. of it, as the four steps' A fragments.  Word
 // s: columns c = 32 (s / 2) + 8 j + 4 (s % 2) ..+3; register i = 0 .. 3 of the
 // fragment has row r + 8 (i & 1) and columns c + 2 (i >> 1), +1, whose codes
-// lie at bits 3 + 4 i (low half) and 19 + 4 i of the word (mod 32).
+// lie at bit 6, 2, 14 and 10 of the word, and 16 higher (mod 32).
 __global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64_t ld, int n, int k, int k_tiles,
                                                       int64_t total, uint4* tiles) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -69,7 +73,8 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64
         const int col = col0 + 32 * (s >> 1) + 8 * j + 4 * (s & 1) + 2 * (i >> 1) + q;
         const int code = row < n && col < k ? codes[row * ld + col] : 0;
         const uint32_t u = static_cast<uint32_t>(code + 8) & 15u;
-        w |= __funnelshift_l(u, u, 3 + 4 * i + 16 * q);  // a rotation: u has four bits
+        const int bit = (i & 1 ? 2 : 6) + (i >> 1) * 8 + 16 * q;
+        w |= __funnelshift_l(u, u, bit);  // a rotation: u has four bits
       }
     words[s] = w;
   }
@@ -78,54 +83,52 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// The A fragment of a word: 1 + u / 16 as bf16 pairs, or q / 16.
-template <bool CENTRED>
+// The A fragment of a word: q / 16 as f16 pairs.
 __device__ __forceinline__ void weights(uint32_t w, uint32_t (&a)[4]) {
-  constexpr uint32_t kMask = 0x00780078u, kOne = 0x3f803f80u;
-  a[0] = (w & kMask) | kOne;
-  a[1] = ((w >> 4) & kMask) | kOne;
-  a[2] = ((w >> 8) & kMask) | kOne;
-  a[3] = (__funnelshift_r(w, w, 12) & kMask) | kOne;
-  if constexpr (CENTRED) {
+  constexpr uint32_t kHigh = 0x03c003c0u, kLow = 0x003c003cu, kOne = 0x3c003c00u;
+  const uint32_t v = __funnelshift_r(w, w, 8);
+  a[0] = (w & kHigh) | kOne;
+  a[1] = (w & kLow) | kOne;
+  a[2] = (v & kHigh) | kOne;
+  a[3] = (v & kLow) | kOne;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      __nv_bfloat162& h = reinterpret_cast<__nv_bfloat162&>(a[i]);
-      h = __hsub2(h, __floats2bfloat162_rn(1.5f, 1.5f));
-    }
+  for (int i = 0; i < 4; ++i) {
+    __half2& h = reinterpret_cast<__half2&>(a[i]);
+    h = i & 1 ? __hfma2(h, __floats2half2_rn(16.f, 16.f), __floats2half2_rn(-16.5f, -16.5f))
+              : __hadd2(h, __floats2half2_rn(-1.5f, -1.5f));
   }
 }
 
-// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns;
-// CENTRED: codes as q / 16 themselves rather than 1.5 + q / 16.
-template <int NT, bool HALVES, bool CENTRED, typename TSc>
-__global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
+// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns.
+template <int NT, bool HALVES, typename TSc>
+__global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
   using Word = typename std::conditional<HALVES, uint2, uint32_t>::type;
-  constexpr int kBlocks = HALVES ? 2 : 1;  // sums of x a k tile
-  constexpr int kCols = 8 * NT;
+  constexpr int kBlocks = HALVES ? 2 : 1;  // powers of two of x a k tile
+  constexpr int kCols = 8 * NT, kThreads = 32 * kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
   extern __shared__ uint4 shared_w4[];
-  __nv_bfloat16* const xs = reinterpret_cast<__nv_bfloat16*>(shared_w4);  // [column][pitch]
+  __half* const xs = reinterpret_cast<__half*>(shared_w4);  // [column][pitch]
 
   const LvsaW4Linear& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
   const int m0 = blockIdx.y * p.pass_rows, rows = min(p.pass_rows, a.m - m0), cols = rows * p.parts;
-  float* const x_sums = reinterpret_cast<float*>(xs + static_cast<int64_t>(p.pass_rows) * p.parts * p.pitch);  // [block][column]
-  float* const joined = x_sums + (CENTRED ? 0 : p.splits * p.chunk * kBlocks * kCols);                        // [warp][column][row]
+  float* const x_scale = reinterpret_cast<float*>(xs + static_cast<int64_t>(p.pass_rows) * p.parts * p.pitch);  // [block][column]
+  float* const joined = x_scale + p.splits * p.chunk * kBlocks * kCols;  // [row of tiles][split][column][row]
   const int split = warp / p.slots, slot = warp - split * p.slots;  // warps beyond splits x slots have nothing
   const int k_first = split * p.stretch, k_last = split < p.splits ? min(p.k_tiles, k_first + p.stretch) : k_first;
   const int scale_words = HALVES ? p.k_tiles : (a.k + a.group - 1) / a.group;  // of a row of tiles, times 8
   const int scale_shift = a.group == 128 ? 1 : 0;
 
-  // x's columns of chunk `first` of every stretch, as bf16 parts, and -1.5
-  // times their sums: a thread takes 8 values, the threads of a block add up.
+  // x's columns of chunk `first` of every stretch, as f16 parts, and their
+  // powers of two: a thread takes 8 values, the threads of a block agree on e.
   auto stage = [&](int first) {
     const int held = p.splits * p.chunk, octets = held * (kTileK / 8);
     constexpr int kLanes = HALVES ? 4 : 8;  // threads a block
-    for (int i = threadIdx.x; i < (rows * octets + 31) / 32 * 32; i += kThreadsW4) {
+    for (int i = threadIdx.x; i < (rows * octets + 31) / 32 * 32; i += kThreads) {
       const int m = i / octets, o = i - m * octets;  // octets is a multiple of 8: a block lies in one row
       const int at = o / 8, stretch = at / p.chunk, tile = first + at - stretch * p.chunk;
       const int64_t k0 = static_cast<int64_t>(stretch * p.stretch + tile) * kTileK + o % 8 * 8;
@@ -141,23 +144,28 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + expf(-v[e]));
       }
+      float most = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+      for (int w = 1; w < kLanes; w <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+      // The largest becomes 2^10 .. 2^11.  Exponents below 11 count as 11.
+      const uint32_t power = min(max(__float_as_uint(most) >> 23, 11u), 254u);
+      const float down = __uint_as_float((264u - power) << 23), up = __uint_as_float((power - 10u) << 23);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= down;
       for (int part = 0; part < p.parts; ++part) {
-        float sum = 0.f;
         uint4 packed;
-        __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(&packed);
+        __half* h = reinterpret_cast<__half*>(&packed);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          h[e] = __float2bfloat16_rn(v[e]);
-          const float back = __bfloat162float(h[e]);
-          v[e] -= back;
-          sum += back;
+          h[e] = __float2half_rn(v[e]);
+          v[e] -= __half2float(h[e]);
         }
         const int c = m * p.parts + part;
-        if (m < rows) *reinterpret_cast<uint4*>(xs + c * p.pitch + 8 * o) = packed;
-        if constexpr (!CENTRED) {
-#pragma unroll
-          for (int w = 1; w < kLanes; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-          if (m < rows && o % kLanes == 0) x_sums[o / kLanes * kCols + c] = -1.5f * sum;
+        if (m < rows) {
+          *reinterpret_cast<uint4*>(xs + c * p.pitch + 8 * o) = packed;
+          if (o % kLanes == 0) x_scale[o / kLanes * kCols + c] = up;
         }
       }
     }
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
     const int c = 8 * t + r;
     x_lane[t] = ((c < cols ? c : 0) * p.pitch + split * p.chunk * kTileK) / 8 + j;
   }
-  const int sums_lane = split * p.chunk * kBlocks * kCols + 2 * j;
+  const int scale_lane = split * p.chunk * kBlocks * kCols + 2 * j;
 
   const bool whole = p.chunk >= p.stretch;
   const int turns = (p.row_tiles + gridDim.x * p.slots - 1) / (gridDim.x * p.slots);
@@ -229,7 +237,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           uint32_t f[4];
-          weights<CENTRED>(words[s], f);
+          weights(words[s], f);
           const bool start = s == 0 || (HALVES && s == 2), stop = s == 3 || (HALVES && s == 1);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -242,14 +250,13 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
             }
             if (stop) {
               const int h = HALVES ? s >> 1 : 0;
-              float2 off = make_float2(0.f, 0.f);
-              if constexpr (!CENTRED) off = *reinterpret_cast<const float2*>(x_sums + sums_lane + (local * kBlocks + h) * kCols + 8 * t);
+              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_lane + (local * kBlocks + h) * kCols + 8 * t);
               const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[h]);
               const float lo = to_f(pair[0]), hi = to_f(pair[1]);
-              acc[t][0] += lo * (part[t][0] + off.x);
-              acc[t][1] += lo * (part[t][1] + off.y);
-              acc[t][2] += hi * (part[t][2] + off.x);
-              acc[t][3] += hi * (part[t][3] + off.y);
+              acc[t][0] += lo * (part[t][0] * up.x);
+              acc[t][1] += lo * (part[t][1] * up.y);
+              acc[t][2] += hi * (part[t][2] * up.x);
+              acc[t][3] += hi * (part[t][3] * up.y);
             }
           }
         }
@@ -275,7 +282,7 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
         if (c < cols && split < p.splits) joined[((slot * p.splits + split) * kCols + c) * kTileN + r + 8 * (i >> 1)] = acc[t][i];
       }
     __syncthreads();
-    for (int i = threadIdx.x; i < p.slots * rows * kTileN; i += kThreadsW4) {
+    for (int i = threadIdx.x; i < p.slots * rows * kTileN; i += kThreads) {
       const int row = i % kTileN, m = i / kTileN % rows, which = i / (kTileN * rows);
       const int64_t n = static_cast<int64_t>((turn * p.slots + which) * gridDim.x + blockIdx.x) * kTileN + row;
       if (n >= a.n) continue;
@@ -292,13 +299,14 @@ __global__ void __launch_bounds__(kThreadsW4, 1) w4_linear_kernel(const __grid_c
 
 // Columns of x lie 64 bytes beyond a multiple of 128 apart: the 8 x 4 lanes' 16 bytes fall on all banks.
 int column_pitch(int tiles) { return tiles * kTileK + 32; }
-int shared_bytes(int nt, bool halves, bool centred, int splits, int slots, int chunk, int cols) {
-  return cols * column_pitch(splits * chunk) * 2 + (centred ? 0 : splits * chunk * (halves ? 2 : 1) * 8 * nt * 4) +
+int shared_bytes(int nt, bool halves, int splits, int slots, int chunk, int cols) {
+  return cols * column_pitch(splits * chunk) * 2 + splits * chunk * (halves ? 2 : 1) * 8 * nt * 4 +
          splits * slots * 8 * nt * kTileN * 4;
 }
 
-template <int NT, bool HALVES, bool CENTRED, typename TSc>
+template <int NT, bool HALVES, typename TSc>
 int launch(W4Params p, cudaStream_t s) {
+  constexpr int kWarps = kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
   p.pass_rows = std::min(p.a.m, 8 * NT / p.parts);
@@ -306,11 +314,11 @@ int launch(W4Params p, cudaStream_t s) {
   // Rows of tiles of an SM; where they are fewer than the warps, more warps share one.
   const int share = (p.row_tiles + ctas - 1) / ctas;
   p.splits = 1;
-  while (2 * p.splits * share <= kWarpsW4 && 2 * p.splits <= p.k_tiles) p.splits *= 2;
+  while (2 * p.splits * share <= kWarps && 2 * p.splits <= p.k_tiles) p.splits *= 2;
   const int cols = p.pass_rows * p.parts;
-  auto shared_of = [&]() { return shared_bytes(NT, HALVES, CENTRED, p.splits, p.slots, p.chunk, cols); };
+  auto shared_of = [&]() { return shared_bytes(NT, HALVES, p.splits, p.slots, p.chunk, cols); };
   for (;; p.splits /= 2) {
-    p.slots = std::min(share, kWarpsW4 / p.splits);
+    p.slots = std::min(share, kWarps / p.splits);
     p.stretch = (p.k_tiles + p.splits - 1) / p.splits;
     // All of x at once where it fits, else a multiple of kAhead tiles of each
     // stretch, which are fewer and longer where even that does not.
@@ -323,25 +331,22 @@ int launch(W4Params p, cudaStream_t s) {
     if (p.splits == 1) return LVSA_ERR_UNSUPPORTED;
   }
   p.pitch = column_pitch(p.splits * p.chunk);
-  auto kern = w4_linear_kernel<NT, HALVES, CENTRED, TSc>;
+  auto kern = w4_linear_kernel<NT, HALVES, TSc>;
   const int shared = shared_of();
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess) return LVSA_ERR_CUDA;
-  kern<<<dim3(std::min(p.row_tiles, ctas), passes), kThreadsW4, shared, s>>>(p);
+  kern<<<dim3(std::min(p.row_tiles, ctas), passes), 32 * kWarps, shared, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-template <bool HALVES, bool CENTRED, typename TSc>
+template <typename TSc>
 int launch_columns(const W4Params& p, cudaStream_t s) {
   const int64_t cols = static_cast<int64_t>(p.a.m) * p.parts;
-  if (cols <= 8) return launch<1, HALVES, CENTRED, TSc>(p, s);
-  return cols <= 16 ? launch<2, HALVES, CENTRED, TSc>(p, s) : launch<4, HALVES, CENTRED, TSc>(p, s);
-}
-
-template <typename TSc>
-int launch_form(const W4Params& p, cudaStream_t s) {
-  const bool centred = p.a.x_dtype == LVSA_DTYPE_F32 || p.a.out_dtype == LVSA_DTYPE_F32;
-  if (p.a.group == 32) return centred ? launch_columns<true, true, TSc>(p, s) : launch_columns<true, false, TSc>(p, s);
-  return centred ? launch_columns<false, true, TSc>(p, s) : launch_columns<false, false, TSc>(p, s);
+  if (p.a.group == 32) {
+    if (cols <= 8) return launch<1, true, TSc>(p, s);
+    return cols <= 16 ? launch<2, true, TSc>(p, s) : launch<4, true, TSc>(p, s);
+  }
+  if (cols <= 8) return launch<1, false, TSc>(p, s);
+  return cols <= 16 ? launch<2, false, TSc>(p, s) : launch<4, false, TSc>(p, s);
 }
 
 }  // namespace
@@ -384,9 +389,10 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   p.a = *a;
   p.k_tiles = (a->k + kTileK - 1) / kTileK;
   p.row_tiles = (a->n + kTileN - 1) / kTileN;
-  p.parts = a->x_dtype == LVSA_DTYPE_F32 ? 3 : a->x_dtype == LVSA_DTYPE_F16 || a->activation != LVSA_W4_ACT_NONE ? 2 : 1;
+  const bool exact = a->x_dtype != LVSA_DTYPE_F32 && a->activation == LVSA_W4_ACT_NONE;
+  p.parts = exact || a->out_dtype == LVSA_DTYPE_BF16 ? 1 : 2;
   p.x_vectors = vector_vector(Vector{a->x, a->ldx, 0, a->x_dtype}, 8);
   if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_form<__nv_bfloat16>(p, s) : launch_form<__half>(p, s);
+  return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_columns<__nv_bfloat16>(p, s) : launch_columns<__half>(p, s);
 }
