@@ -371,9 +371,9 @@ int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
  * lvsa_w4_pack lays codes [n, k] (int8, row stride ld) out once, into
  * lvsa_w4_bytes bytes: tiles of 16 rows x 64 columns, 512 bytes each, the
  * tiles of a row of tiles side by side; rows and columns past the end hold
- * code 0.  `scales`: with T = ceil(k / 64) and words of two 2-byte scales (rows
- * r and r + 8 of a tile), [ceil(n / 16)][ceil(k / group)][8] words for group 64
- * or 128 and [ceil(n / 16)][T][8][2] words for group 32, 0 past the end.
+ * code 0.  `scales`: [ceil(n / 16)][ceil(k / 64)][8][G] words of two 2-byte
+ * scales (rows r and r + 8 of a tile), G = 2 for group 32 and 1 otherwise (group
+ * 128: each scale twice), 0 past the end.
  *
  * Products are exact and sums fp32, with one rounding to the output's type; x
  * enters as f16 parts of 64 (32) values over their power of two, 11 bits where

@@ -35,9 +35,9 @@ namespace {
 constexpr int kTileN = 16, kTileK = 64;
 constexpr int kMaxShared = 227 * 1024 - 1024;
 // Warps of a CTA, and tiles of a warp on their way: as many warps as the
-// registers allow, 32 with one tile of columns.
+// registers allow, 28 (of 72) with one tile of columns.
 template <int NT>
-constexpr int kWarpsW4 = NT == 1 ? 32 : 16;
+constexpr int kWarpsW4 = NT == 1 ? 28 : 16;
 template <int NT>
 constexpr int kAhead = NT == 1 ? 4 : 8;
 
@@ -82,8 +82,7 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64
 }
 
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
@@ -120,8 +119,6 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
   float* const joined = x_scale + p.splits * p.chunk * kBlocks * kCols;  // [row of tiles][split][column][row]
   const int split = warp / p.slots, slot = warp - split * p.slots;  // warps beyond splits x slots have nothing
   const int k_first = split * p.stretch, k_last = split < p.splits ? min(p.k_tiles, k_first + p.stretch) : k_first;
-  const int scale_words = HALVES ? p.k_tiles : (a.k + a.group - 1) / a.group;  // of a row of tiles, times 8
-  const int scale_shift = a.group == 128 ? 1 : 0;
 
   // x's columns of chunk `first` of every stretch, as f16 parts, and their
   // powers of two: a thread takes 8 values, the threads of a block agree on e.
@@ -188,15 +185,15 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
     // Neighbouring CTAs take neighbouring rows of tiles: the SMs' shares differ by one at most.
     const int row_tile = (turn * p.slots + slot) * gridDim.x + blockIdx.x;
     const int last = row_tile < p.row_tiles ? k_last : k_first;
-    const uint4* tiles = static_cast<const uint4*>(a.tiles) + static_cast<int64_t>(row_tile) * p.k_tiles * 32 + lane;
-    const Word* scales = static_cast<const Word*>(a.scales) + static_cast<int64_t>(row_tile) * scale_words * 8 + r;
+    const uint4* tiles = static_cast<const uint4*>(a.tiles) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 32 + lane;
+    const Word* scales = static_cast<const Word*>(a.scales) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 8 + r;
     uint4 w[kAhead];
     Word sc[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (k_first + u < last) {
-        w[u] = __ldg(tiles + (k_first + u) * 32);
-        sc[u] = __ldg(scales + ((k_first + u) >> scale_shift) * 8);
+        w[u] = __ldg(tiles + u * 32);
+        sc[u] = __ldg(scales + u * 8);
       }
     float acc[NT][4];
 #pragma unroll
@@ -211,20 +208,23 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
         __syncthreads();
       }
       const int end = min(last, k_first + first + p.chunk);
-      // One tile from w[u], in whose place the one kAhead later is asked for.
-      auto tile_of = [&](int tile, int u, bool more) {
+      int x_at[NT], scale_at = scale_lane;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) x_at[t] = x_lane[t];
+      // The u-th of kAhead tiles, from w[u], in whose place the one kAhead
+      // later is asked for.
+      auto tile_of = [&](int u, bool more) {
         const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
         const Word word = sc[u];
         if (more) {
-          w[u] = __ldg(tiles + (tile + kAhead) * 32);
-          sc[u] = __ldg(scales + ((tile + kAhead) >> scale_shift) * 8);
+          w[u] = __ldg(tiles + (u + kAhead) * 32);
+          sc[u] = __ldg(scales + (u + kAhead) * 8);
         }
-        const int local = tile - k_first - first;
         uint4 b[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          b[t][0] = shared_w4[x_lane[t] + local * (kTileK / 8)];
-          b[t][1] = shared_w4[x_lane[t] + local * (kTileK / 8) + 4];
+          b[t][0] = shared_w4[x_at[t] + u * (kTileK / 8)];
+          b[t][1] = shared_w4[x_at[t] + u * (kTileK / 8) + 4];
         }
         uint32_t scale_pairs[kBlocks];
         if constexpr (HALVES) {
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
             }
             if (stop) {
               const int h = HALVES ? s >> 1 : 0;
-              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_lane + (local * kBlocks + h) * kCols + 8 * t);
+              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + h) * kCols + 8 * t);
               const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[h]);
               const float lo = to_f(pair[0]), hi = to_f(pair[1]);
               acc[t][0] += lo * (part[t][0] * up.x);
@@ -261,15 +261,24 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
           }
         }
       };
+      auto on = [&]() {
+        tiles += kAhead * 32;
+        scales += kAhead * 8;
+        scale_at += kAhead * kBlocks * kCols;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) x_at[t] += kAhead * (kTileK / 8);
+      };
       int base = k_first + first;
       for (; base + 2 * kAhead <= last && base + kAhead <= end; base += kAhead) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) tile_of(base + u, u, true);
+        for (int u = 0; u < kAhead; ++u) tile_of(u, true);
+        on();
       }
       for (; base < end; base += kAhead) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-          if (base + u < end) tile_of(base + u, u, base + u + kAhead < last);
+          if (base + u < end) tile_of(u, base + u + kAhead < last);
+        on();
       }
     }
     // Join the stretches and the parts: [row of tiles of the CTA][split][column][row].
@@ -313,13 +322,13 @@ int launch(W4Params p, cudaStream_t s) {
   const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows, ctas = std::max(1, sms / passes);
   // Rows of tiles of an SM; where they are fewer than the warps, more warps share one.
   const int share = (p.row_tiles + ctas - 1) / ctas;
-  p.splits = 1;
-  while (2 * p.splits * share <= kWarps && 2 * p.splits <= p.k_tiles) p.splits *= 2;
+  p.splits = std::max(1, std::min(kWarps / share, p.k_tiles));
   const int cols = p.pass_rows * p.parts;
   auto shared_of = [&]() { return shared_bytes(NT, HALVES, p.splits, p.slots, p.chunk, cols); };
   for (;; p.splits /= 2) {
-    p.slots = std::min(share, kWarps / p.splits);
     p.stretch = (p.k_tiles + p.splits - 1) / p.splits;
+    p.splits = (p.k_tiles + p.stretch - 1) / p.stretch;
+    p.slots = std::min(share, kWarps / p.splits);
     // All of x at once where it fits, else a multiple of kAhead tiles of each
     // stretch, which are fewer and longer where even that does not.
     p.chunk = p.stretch;

@@ -68,14 +68,12 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, group: int) -> W4Weight:
     with torch.cuda.device(codes.device):
         st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0), n, k, tiles.data_ptr(), _stream_ptr(codes.device))
     N.check(st, "lvsa_w4_pack")
-    rows, blocks = -(-n // 16), -(-k // group)
-    if group == 32:
-        blocks = -(-k // 64) * 2
-    s = torch.nn.functional.pad(scales.detach(), (0, blocks - scales.shape[1], 0, rows * 16 - n)).view(rows, 2, 8, blocks)
-    if group == 32:  # [row of tiles, k tile, row, half, row or row + 8]
-        s = s.unflatten(3, (-1, 2)).permute(0, 3, 2, 4, 1)
-    else:            # [row of tiles, group, row, row or row + 8]
-        s = s.permute(0, 3, 2, 1)
+    # Two words a tile of 64 columns for group 32, one otherwise; a word has rows r and r + 8.
+    rows, tile = -(-n // 16), max(1, 64 // group)
+    s = scales.detach().repeat_interleave(2, dim=1) if group == 128 else scales.detach()
+    s = s[:, :-(-k // 64) * tile]
+    s = torch.nn.functional.pad(s, (0, -(-k // 64) * tile - s.shape[1], 0, rows * 16 - n))
+    s = s.view(rows, 2, 8, -1, tile).permute(0, 3, 2, 4, 1)
     return W4Weight(n, k, group, tiles, s.contiguous())
 
 
