@@ -375,10 +375,9 @@ int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
  * scales (rows r and r + 8 of a tile), G = 2 for group 32 and 1 otherwise (group
  * 128: each scale twice), 0 past the end.
  *
- * Products are exact and sums fp32, with one rounding to the output's type; x
- * enters as f16 parts of 64 (32) values over their power of two, 11 bits where
- * x has no more or the output is bf16, else 22.  A row of x that holds an
- * infinity or NaN gives infinities or NaN. */
+ * The values of x that one scale goes with count to 2^-22 of their largest;
+ * products with codes are exact, sums fp32, with one rounding to the output's
+ * type.  A row of x that holds an infinity or NaN gives NaN. */
 enum { LVSA_W4_ACT_NONE = 0, LVSA_W4_ACT_SILU = 1 };
 typedef struct LvsaW4Linear {
   const void* x;     /* [m, k], row stride ldx elements, bf16 / f16 / fp32       */

@@ -2,18 +2,18 @@
 // rows of x: out[m, n] = sum_k act(x[m, k]) s[n, k / group] q[n, k] (+ bias).
 // Bound: HBM, n k / 2 bytes of codes and 2 n k / group of scales read once.
 //
-// Arithmetic.  A code q = -8 .. 7 is stored as u = q + 8.  Set into an f16
-// number's mantissa at its top, u makes 1 + u / 16, four bits lower 1 + u / 256;
-// one half-precision operation takes either to q / 16, exactly, so that two
-// codes cost 1.25 integer operations (the pipe that bounds this kernel next to
-// HBM) and one on the other pipe.  m16n8k16 multiplies (weights as its 16 rows,
-// parts of rows of x as its 8 columns; f16 products are exact, sums fp32).
-// x enters as f16 parts, one or two (11 or 22 bits), of x / 2^e, with e of the
-// largest of the 64 (32) values that one scale of the weights goes with: 2^e
-// joins that scale in fp32, and any x fits f16's range.  One part where that is
-// exact (a 16-bit x without an activation) or where the result is bf16 (2^-12
-// of x under 2^-9 of the result), two otherwise; with few rows the columns
-// are free.
+// Arithmetic, on the 8-bit integer tensor cores.  Codes go in as 16 q, one
+// byte each: eight lie in a 32-bit word so that the high and the low half of
+// its bytes are one AND, and one shift and AND, away (the integer pipe bounds
+// this kernel next to HBM: f16 weights took 36 operations a tile of 16 x 64,
+// these take 12).  The 64 (32) values of x that one scale of the weights goes
+// with become whole numbers of 23 bits and sign, their largest 2^21 .. 2^22 by
+// a power of two, in three signed digits of 8 bits: m16n8k32 multiplies them,
+// weights as its 16 rows, digits of rows of x as its 8 columns, without any
+// rounding, and starts from 1.5 2^23 as a float's bits, so that the sum is a
+// float after one subtraction.  Scale, digit's place and power of two join it
+// in fp32.  So x counts to 2^-22 of the largest of its neighbours, as sums in
+// fp32 count, whatever its type.
 //
 // Work.  A CTA an SM, 16 warps; x, as parts, in its shared memory.  A warp
 // takes a row of tiles (16 rows of weights), or one of `splits` stretches of
@@ -43,85 +43,67 @@ constexpr int kAhead = NT == 1 ? 4 : 8;
 
 struct W4Params {
   LvsaW4Linear a;
-  int32_t k_tiles, row_tiles, parts;
+  int32_t k_tiles, row_tiles;
   int32_t pass_rows;      // rows of x a pass (blockIdx.y)
   int32_t splits, slots;  // stretches of a row of tiles; rows of tiles of a CTA at once
   int32_t stretch;        // k tiles of a stretch
   int32_t chunk;          // k tiles of each stretch for which x is held at once
-  int32_t pitch;          // bf16 values between the columns of x held
+  int32_t pitch;          // 16 bytes between the columns of x held
   int32_t x_vectors;      // x may be read 8 values at a time
 };
 
 // ---- layout: lane l = 4 r + j of a tile holds rows r and r + 8, columns
-// 8 j .. 8 j + 7 and 32 + 8 j .. of it, as the four steps' A fragments.  Word
-// s: columns c = 32 (s / 2) + 8 j + 4 (s % 2) ..+3; register i = 0 .. 3 of the
-// fragment has row r + 8 (i & 1) and columns c + 2 (i >> 1), +1, whose codes
-// lie at bit 6, 2, 14 and 10 of the word, and 16 higher (mod 32).
+// 8 j .. 8 j + 7 and 32 + 8 j .. of it.  Byte i of word 2 s + h has column
+// 32 s + 8 j + 4 h + i: row r in its high half, row r + 8 in its low one.
 __global__ void __launch_bounds__(256) w4_pack_kernel(const int8_t* codes, int64_t ld, int n, int k, int k_tiles,
                                                       int64_t total, uint4* tiles) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= total) return;
   const int lane = at & 31, r = lane >> 2, j = lane & 3;
-  const int64_t tile = at >> 5, row0 = tile / k_tiles * kTileN;
-  const int col0 = static_cast<int>(tile % k_tiles) * kTileK;
+  const int64_t tile = at >> 5, row = tile / k_tiles * kTileN + r;
+  const int col0 = static_cast<int>(tile % k_tiles) * kTileK + 8 * j;
   uint32_t words[4];
-  for (int s = 0; s < 4; ++s) {
-    uint32_t w = 0;
-    for (int i = 0; i < 4; ++i)
-      for (int q = 0; q < 2; ++q) {
-        const int64_t row = row0 + r + 8 * (i & 1);
-        const int col = col0 + 32 * (s >> 1) + 8 * j + 4 * (s & 1) + 2 * (i >> 1) + q;
-        const int code = row < n && col < k ? codes[row * ld + col] : 0;
-        const uint32_t u = static_cast<uint32_t>(code + 8) & 15u;
-        const int bit = (i & 1 ? 2 : 6) + (i >> 1) * 8 + 16 * q;
-        w |= __funnelshift_l(u, u, bit);  // a rotation: u has four bits
-      }
-    words[s] = w;
+  for (int w = 0; w < 4; ++w) {
+    words[w] = 0;
+    for (int i = 0; i < 4; ++i) {
+      const int col = col0 + 32 * (w >> 1) + 4 * (w & 1) + i;
+      const uint32_t high = row < n && col < k ? codes[row * ld + col] & 15 : 0;
+      const uint32_t low = row + 8 < n && col < k ? codes[(row + 8) * ld + col] & 15 : 0;
+      words[w] |= (high << 4 | low) << (8 * i);
+    }
   }
   tiles[at] = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+__device__ __forceinline__ void mma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const int (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
+constexpr int kDigits = 3;
+constexpr int kMagic = 0x4b400000;  // 1.5 2^23: a sum of at most 64 x 128 x 128 = 2^20 leaves its exponent
+constexpr float kMagicValue = 12582912.f;
 
-// The A fragment of a word: q / 16 as f16 pairs.
-__device__ __forceinline__ void weights(uint32_t w, uint32_t (&a)[4]) {
-  constexpr uint32_t kHigh = 0x03c003c0u, kLow = 0x003c003cu, kOne = 0x3c003c00u;
-  const uint32_t v = __funnelshift_r(w, w, 8);
-  a[0] = (w & kHigh) | kOne;
-  a[1] = (w & kLow) | kOne;
-  a[2] = (v & kHigh) | kOne;
-  a[3] = (v & kLow) | kOne;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    __half2& h = reinterpret_cast<__half2&>(a[i]);
-    h = i & 1 ? __hfma2(h, __floats2half2_rn(16.f, 16.f), __floats2half2_rn(-16.5f, -16.5f))
-              : __hadd2(h, __floats2half2_rn(-1.5f, -1.5f));
-  }
-}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
-// NT: column tiles of 8 (parts of rows of x); HALVES: groups of 32 columns.
+// NT: column tiles of 8 (digits of rows of x); HALVES: groups of 32 columns.
 template <int NT, bool HALVES, typename TSc>
 __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
   using Word = typename std::conditional<HALVES, uint2, uint32_t>::type;
   constexpr int kBlocks = HALVES ? 2 : 1;  // powers of two of x a k tile
   constexpr int kCols = 8 * NT, kThreads = 32 * kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
   extern __shared__ uint4 shared_w4[];
-  __half* const xs = reinterpret_cast<__half*>(shared_w4);  // [column][pitch]
 
   const LvsaW4Linear& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, j = lane & 3;
-  const int m0 = blockIdx.y * p.pass_rows, rows = min(p.pass_rows, a.m - m0), cols = rows * p.parts;
-  float* const x_scale = reinterpret_cast<float*>(xs + static_cast<int64_t>(p.pass_rows) * p.parts * p.pitch);  // [block][column]
+  const int m0 = blockIdx.y * p.pass_rows, rows = min(p.pass_rows, a.m - m0), cols = rows * kDigits;
+  float* const x_scale = reinterpret_cast<float*>(shared_w4 + p.pass_rows * kDigits * p.pitch);  // [block][column], after x's [column][pitch]
   float* const joined = x_scale + p.splits * p.chunk * kBlocks * kCols;  // [row of tiles][split][column][row]
   const int split = warp / p.slots, slot = warp - split * p.slots;  // warps beyond splits x slots have nothing
   const int k_first = split * p.stretch, k_last = split < p.splits ? min(p.k_tiles, k_first + p.stretch) : k_first;
 
-  // x's columns of chunk `first` of every stretch, as f16 parts, and their
-  // powers of two: a thread takes 8 values, the threads of a block agree on e.
+  // x's columns of chunk `first` of every stretch, as digits, and their powers
+  // of two: a thread takes 8 values, the threads of a block agree on a power.
   auto stage = [&](int first) {
     const int held = p.splits * p.chunk, octets = held * (kTileK / 8);
     constexpr int kLanes = HALVES ? 4 : 8;  // threads a block
@@ -141,29 +123,34 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + expf(-v[e]));
       }
-      float most = 0.f;
+      uint32_t most = 0;  // of the sizes' bits: a NaN is larger than all
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+      for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
 #pragma unroll
-      for (int w = 1; w < kLanes; w <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
-      // The largest becomes 2^10 .. 2^11.  Exponents below 11 count as 11.
-      const uint32_t power = min(max(__float_as_uint(most) >> 23, 11u), 254u);
-      const float down = __uint_as_float((264u - power) << 23), up = __uint_as_float((power - 10u) << 23);
+      for (int w = 1; w < kLanes; w <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, w));
+      // Exponents below 26 count as 26: smaller values than 2^-123 are lost.
+      const uint32_t power = min(max(most >> 23, 26u), 254u);
+      const float down = __uint_as_float((275u - power) << 23);
+      // 2^-16 for the codes' 16; infinities and NaN make the row NaN.
+      float up = most < 0x7f800000u ? __uint_as_float((power - 25u) << 23) : __uint_as_float(0x7fc00000u);
+      int whole[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= down;
-      for (int part = 0; part < p.parts; ++part) {
-        uint4 packed;
-        __half* h = reinterpret_cast<__half*>(&packed);
+      for (int e = 0; e < 8; ++e) whole[e] = __float2int_rn(v[e] * down);
+#pragma unroll
+      for (int digit = 0; digit < kDigits; ++digit) {
+        uint32_t packed[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          h[e] = __float2half_rn(v[e]);
-          v[e] -= __half2float(h[e]);
+          const int d = static_cast<int8_t>(whole[e]);
+          packed[e >> 2] |= (static_cast<uint32_t>(d) & 255u) << (8 * (e & 3));
+          whole[e] = (whole[e] - d) >> 8;
         }
-        const int c = m * p.parts + part;
-        if (m < rows) {
-          *reinterpret_cast<uint4*>(xs + c * p.pitch + 8 * o) = packed;
+        const int c = m * kDigits + digit;
+        if (m < rows) {  // lane j's 16 bytes: its 8 columns of either half of the tile
+          reinterpret_cast<uint2*>(shared_w4 + c * p.pitch + at * 4 + o % 4)[o / 4 % 2] = make_uint2(packed[0], packed[1]);
           if (o % kLanes == 0) x_scale[o / kLanes * kCols + c] = up;
         }
+        up *= 256.f;
       }
     }
   };
@@ -175,7 +162,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int c = 8 * t + r;
-    x_lane[t] = ((c < cols ? c : 0) * p.pitch + split * p.chunk * kTileK) / 8 + j;
+    x_lane[t] = (c < cols ? c : 0) * p.pitch + split * p.chunk * 4 + j;
   }
   const int scale_lane = split * p.chunk * kBlocks * kCols + 2 * j;
 
@@ -187,6 +174,10 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
     const int last = row_tile < p.row_tiles ? k_last : k_first;
     const uint4* tiles = static_cast<const uint4*>(a.tiles) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 32 + lane;
     const Word* scales = static_cast<const Word*>(a.scales) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 8 + r;
+    if (turn == 0) {  // the rest of the stretch on its way to L2 while x is made ready
+      const char* from = reinterpret_cast<const char*>(tiles - lane);
+      for (int at = kAhead * 512 + lane * 128; at < (last - k_first) * 512; at += 32 * 128) prefetch_l2(from + at);
+    }
     uint4 w[kAhead];
     Word sc[kAhead];
 #pragma unroll
@@ -216,16 +207,9 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       auto tile_of = [&](int u, bool more) {
         const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
         const Word word = sc[u];
-        if (more) {
-          w[u] = __ldg(tiles + (u + kAhead) * 32);
-          sc[u] = __ldg(scales + (u + kAhead) * 8);
-        }
-        uint4 b[NT][2];
+        uint4 b[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          b[t][0] = shared_w4[x_at[t] + u * (kTileK / 8)];
-          b[t][1] = shared_w4[x_at[t] + u * (kTileK / 8) + 4];
-        }
+        for (int t = 0; t < NT; ++t) b[t] = shared_w4[x_at[t] + u * 4];
         uint32_t scale_pairs[kBlocks];
         if constexpr (HALVES) {
           scale_pairs[0] = word.x;
@@ -233,32 +217,34 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
         } else {
           scale_pairs[0] = word;
         }
-        float part[NT][4];
+        int sum[NT][4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          uint32_t f[4];
-          weights(words[s], f);
-          const bool start = s == 0 || (HALVES && s == 2), stop = s == 3 || (HALVES && s == 1);
+        for (int h = 0; h < 2; ++h) {  // halves of the tile
+          constexpr uint32_t kHigh = 0xf0f0f0f0u;
+          const uint32_t f[4] = {words[2 * h] & kHigh, words[2 * h] << 4 & kHigh, words[2 * h + 1] & kHigh,
+                                 words[2 * h + 1] << 4 & kHigh};
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const uint4& q = b[t][s >> 1];
-            if (start) {
-              const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-              mma(part[t], f, s & 1 ? q.z : q.x, s & 1 ? q.w : q.y, zero);
+            if (h == 0 || HALVES) {
+              const int magic[4] = {kMagic, kMagic, kMagic, kMagic};
+              mma(sum[t], f, h ? b[t].z : b[t].x, h ? b[t].w : b[t].y, magic);
             } else {
-              mma(part[t], f, s & 1 ? q.z : q.x, s & 1 ? q.w : q.y, part[t]);
+              mma(sum[t], f, b[t].z, b[t].w, sum[t]);
             }
-            if (stop) {
-              const int h = HALVES ? s >> 1 : 0;
-              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + h) * kCols + 8 * t);
-              const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[h]);
+            if (h == 1 || HALVES) {
+              const int block = HALVES ? h : 0;
+              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * t);
+              const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[block]);
               const float lo = to_f(pair[0]), hi = to_f(pair[1]);
-              acc[t][0] += lo * (part[t][0] * up.x);
-              acc[t][1] += lo * (part[t][1] * up.y);
-              acc[t][2] += hi * (part[t][2] * up.x);
-              acc[t][3] += hi * (part[t][3] * up.y);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[t][i] += (i < 2 ? lo : hi) * ((__int_as_float(sum[t][i]) - kMagicValue) * (i & 1 ? up.y : up.x));
             }
           }
+        }
+        if (more) {
+          w[u] = __ldg(tiles + (u + kAhead) * 32);
+          sc[u] = __ldg(scales + (u + kAhead) * 8);
         }
       };
       auto on = [&]() {
@@ -266,7 +252,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
         scales += kAhead * 8;
         scale_at += kAhead * kBlocks * kCols;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) x_at[t] += kAhead * (kTileK / 8);
+        for (int t = 0; t < NT; ++t) x_at[t] += kAhead * 4;
       };
       int base = k_first + first;
       for (; base + 2 * kAhead <= last && base + kAhead <= end; base += kAhead) {
@@ -281,7 +267,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
         on();
       }
     }
-    // Join the stretches and the parts: [row of tiles of the CTA][split][column][row].
+    // Join the stretches and the digits: [row of tiles of the CTA][split][column][row].
     if (turn > 0) __syncthreads();  // the turn before has been read
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -296,20 +282,19 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       const int64_t n = static_cast<int64_t>((turn * p.slots + which) * gridDim.x + blockIdx.x) * kTileN + row;
       if (n >= a.n) continue;
       float sum = 0.f;
-      for (int part = p.parts - 1; part >= 0; --part)  // the small parts first
+      for (int digit = 0; digit < kDigits; ++digit)
         for (int s = 0; s < p.splits; ++s)
-          sum += joined[((which * p.splits + s) * kCols + m * p.parts + part) * kTileN + row];
-      sum *= 16.f;
+          sum += joined[((which * p.splits + s) * kCols + m * kDigits + digit) * kTileN + row];
       if (a.bias) sum += any_load(a.bias, a.bias_dtype, n);
       any_store(a.out, a.out_dtype, (m0 + m) * a.ldo + n, sum);
     }
   }
 }
 
-// Columns of x lie 64 bytes beyond a multiple of 128 apart: the 8 x 4 lanes' 16 bytes fall on all banks.
-int column_pitch(int tiles) { return tiles * kTileK + 32; }
+// Columns of x lie an odd multiple of 64 bytes apart: the 8 x 4 lanes' 16 bytes fall on all banks.
+int column_pitch(int tiles) { return (tiles * kTileK + 63) / 128 * 8 + 4; }  // of 16 bytes
 int shared_bytes(int nt, bool halves, int splits, int slots, int chunk, int cols) {
-  return cols * column_pitch(splits * chunk) * 2 + splits * chunk * (halves ? 2 : 1) * 8 * nt * 4 +
+  return cols * column_pitch(splits * chunk) * 16 + splits * chunk * (halves ? 2 : 1) * 8 * nt * 4 +
          splits * slots * 8 * nt * kTileN * 4;
 }
 
@@ -318,12 +303,12 @@ int launch(W4Params p, cudaStream_t s) {
   constexpr int kWarps = kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
-  p.pass_rows = std::min(p.a.m, 8 * NT / p.parts);
+  p.pass_rows = std::min(p.a.m, 8 * NT / kDigits);
   const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows, ctas = std::max(1, sms / passes);
   // Rows of tiles of an SM; where they are fewer than the warps, more warps share one.
   const int share = (p.row_tiles + ctas - 1) / ctas;
   p.splits = std::max(1, std::min(kWarps / share, p.k_tiles));
-  const int cols = p.pass_rows * p.parts;
+  const int cols = p.pass_rows * kDigits;
   auto shared_of = [&]() { return shared_bytes(NT, HALVES, p.splits, p.slots, p.chunk, cols); };
   for (;; p.splits /= 2) {
     p.stretch = (p.k_tiles + p.splits - 1) / p.splits;
@@ -349,7 +334,7 @@ int launch(W4Params p, cudaStream_t s) {
 
 template <typename TSc>
 int launch_columns(const W4Params& p, cudaStream_t s) {
-  const int64_t cols = static_cast<int64_t>(p.a.m) * p.parts;
+  const int64_t cols = static_cast<int64_t>(p.a.m) * kDigits;
   if (p.a.group == 32) {
     if (cols <= 8) return launch<1, true, TSc>(p, s);
     return cols <= 16 ? launch<2, true, TSc>(p, s) : launch<4, true, TSc>(p, s);
@@ -398,8 +383,6 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   p.a = *a;
   p.k_tiles = (a->k + kTileK - 1) / kTileK;
   p.row_tiles = (a->n + kTileN - 1) / kTileN;
-  const bool exact = a->x_dtype != LVSA_DTYPE_F32 && a->activation == LVSA_W4_ACT_NONE;
-  p.parts = exact || a->out_dtype == LVSA_DTYPE_BF16 ? 1 : 2;
   p.x_vectors = vector_vector(Vector{a->x, a->ldx, 0, a->x_dtype}, 8);
   if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -99,11 +99,11 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     """act(x) W^T + bias: x [..., k] -> [..., n] in ``out_dtype`` (default x's).
 
     x, bias and output in bf16, fp16 or fp32; ``activation`` None or "silu",
-    in fp32.  Products are exact and sums fp32, with one rounding of the
-    result; act(x) counts with 11 bits where it has no more or the output is
-    bf16, else with 22.  Made for few rows (a row a sequence or a latent
-    frame): each further 32 (16 with 22 bits) read the weights once more.
-    Inference only: x must not require grad."""
+    in fp32.  Values of act(x) count to 2^-22 of the largest of the 64 (32) in
+    their group; products with codes are exact and sums fp32, with one
+    rounding of the result.  A row with an infinity or NaN gives NaN.  Made for
+    few rows (a row a sequence or a latent frame): each further 10 read the
+    weights once more.  Inference only: x must not require grad."""
     if not x.is_cuda:
         raise RuntimeError("linear_w4 needs CUDA tensors (no CPU fallback)")
     out_dtype = x.dtype if out_dtype is None else out_dtype
