@@ -34,12 +34,13 @@ namespace {
 
 constexpr int kTileN = 16, kTileK = 64;
 constexpr int kMaxShared = 227 * 1024 - 1024;
-// Warps of a CTA, and tiles of a warp on their way: as many warps as the
-// registers allow, 28 (of 72) with one tile of columns.
+// Warps of a CTA, as many as the registers allow, and tiles of a warp on their
+// way.  One row of 30720 x 5120: 28 warps with 4 tiles 18.9 us, with 3 19.4, 5
+// 19.7, 6 19.9; 32 with 4 19.8, with 3 20.3; prefetching further to L2 is slower
+// (8 tiles more 20.6, 16 22.0).
 template <int NT>
-constexpr int kWarpsW4 = NT == 1 ? 28 : 16;
-template <int NT>
-constexpr int kAhead = NT == 1 ? 4 : 8;
+constexpr int kWarpsW4 = NT <= 4 ? 28 : 20;
+constexpr int kAhead = 4;
 
 struct W4Params {
   LvsaW4Linear a;
@@ -84,14 +85,12 @@ constexpr int kDigits = 3;
 constexpr int kMagic = 0x4b400000;  // 1.5 2^23: a sum of at most 64 x 128 x 128 = 2^20 leaves its exponent
 constexpr float kMagicValue = 12582912.f;
 
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
-
 // NT: column tiles of 8 (digits of rows of x); HALVES: groups of 32 columns.
 template <int NT, bool HALVES, typename TSc>
 __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const __grid_constant__ W4Params p) {
   using Word = typename std::conditional<HALVES, uint2, uint32_t>::type;
   constexpr int kBlocks = HALVES ? 2 : 1;  // powers of two of x a k tile
-  constexpr int kCols = 8 * NT, kThreads = 32 * kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
+  constexpr int kCols = 8 * NT, kThreads = 32 * kWarpsW4<NT>;
   extern __shared__ uint4 shared_w4[];
 
   const LvsaW4Linear& a = p.a;
@@ -121,7 +120,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       }
       if (a.activation == LVSA_W4_ACT_SILU) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = v[e] / (1.f + expf(-v[e]));
+        for (int e = 0; e < 8; ++e) v[e] = __fdividef(v[e], 1.f + expf(-v[e]));  // past 2^126: 0
       }
       uint32_t most = 0;  // of the sizes' bits: a NaN is larger than all
 #pragma unroll
@@ -133,17 +132,20 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       const float down = __uint_as_float((275u - power) << 23);
       // 2^-16 for the codes' 16; infinities and NaN make the row NaN.
       float up = most < 0x7f800000u ? __uint_as_float((power - 25u) << 23) : __uint_as_float(0x7fc00000u);
-      int whole[8];
+      // Rounded to a whole number by 1.5 2^23, and with 128 (1 + 256 + 65536)
+      // more, the bytes of it are the digits + 128.
+      uint32_t whole[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) whole[e] = __float2int_rn(v[e] * down);
+      for (int e = 0; e < 8; ++e)
+        whole[e] = (__float_as_uint(fmaf(v[e], down, kMagicValue)) - (kMagic - 0x00808080u)) ^ 0x00808080u;
 #pragma unroll
       for (int digit = 0; digit < kDigits; ++digit) {
-        uint32_t packed[2] = {0u, 0u};
+        uint32_t packed[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = static_cast<int8_t>(whole[e]);
-          packed[e >> 2] |= (static_cast<uint32_t>(d) & 255u) << (8 * (e & 3));
-          whole[e] = (whole[e] - d) >> 8;
+        for (int q = 0; q < 2; ++q) {  // byte `digit` of four numbers
+          const uint32_t pick = digit | (digit + 4) << 4;
+          packed[q] = __byte_perm(__byte_perm(whole[4 * q], whole[4 * q + 1], pick),
+                                  __byte_perm(whole[4 * q + 2], whole[4 * q + 3], pick), 0x5410);
         }
         const int c = m * kDigits + digit;
         if (m < rows) {  // lane j's 16 bytes: its 8 columns of either half of the tile
@@ -164,6 +166,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
     const int c = 8 * t + r;
     x_lane[t] = (c < cols ? c : 0) * p.pitch + split * p.chunk * 4 + j;
   }
+  const int column_tiles = (cols + 7) / 8;
   const int scale_lane = split * p.chunk * kBlocks * kCols + 2 * j;
 
   const bool whole = p.chunk >= p.stretch;
@@ -174,10 +177,6 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
     const int last = row_tile < p.row_tiles ? k_last : k_first;
     const uint4* tiles = static_cast<const uint4*>(a.tiles) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 32 + lane;
     const Word* scales = static_cast<const Word*>(a.scales) + (static_cast<int64_t>(row_tile) * p.k_tiles + k_first) * 8 + r;
-    if (turn == 0) {  // the rest of the stretch on its way to L2 while x is made ready
-      const char* from = reinterpret_cast<const char*>(tiles - lane);
-      for (int at = kAhead * 512 + lane * 128; at < (last - k_first) * 512; at += 32 * 128) prefetch_l2(from + at);
-    }
     uint4 w[kAhead];
     Word sc[kAhead];
 #pragma unroll
@@ -207,9 +206,6 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       auto tile_of = [&](int u, bool more) {
         const uint32_t words[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
         const Word word = sc[u];
-        uint4 b[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) b[t] = shared_w4[x_at[t] + u * 4];
         uint32_t scale_pairs[kBlocks];
         if constexpr (HALVES) {
           scale_pairs[0] = word.x;
@@ -217,29 +213,40 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
         } else {
           scale_pairs[0] = word;
         }
-        int sum[NT][4];
+        float lo[kBlocks], hi[kBlocks];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // halves of the tile
-          constexpr uint32_t kHigh = 0xf0f0f0f0u;
-          const uint32_t f[4] = {words[2 * h] & kHigh, words[2 * h] << 4 & kHigh, words[2 * h + 1] & kHigh,
-                                 words[2 * h + 1] << 4 & kHigh};
+        for (int block = 0; block < kBlocks; ++block) {
+          const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[block]);
+          lo[block] = to_f(pair[0]);
+          hi[block] = to_f(pair[1]);
+        }
+        constexpr uint32_t kHigh = 0xf0f0f0f0u;
+        uint32_t f[2][4];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (h == 0 || HALVES) {
-              const int magic[4] = {kMagic, kMagic, kMagic, kMagic};
-              mma(sum[t], f, h ? b[t].z : b[t].x, h ? b[t].w : b[t].y, magic);
-            } else {
-              mma(sum[t], f, b[t].z, b[t].w, sum[t]);
-            }
-            if (h == 1 || HALVES) {
-              const int block = HALVES ? h : 0;
-              const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * t);
-              const TSc* pair = reinterpret_cast<const TSc*>(&scale_pairs[block]);
-              const float lo = to_f(pair[0]), hi = to_f(pair[1]);
+        for (int h = 0; h < 4; ++h) {
+          f[h >> 1][2 * (h & 1)] = words[h] & kHigh;
+          f[h >> 1][2 * (h & 1) + 1] = words[h] << 4 & kHigh;
+        }
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[t][i] += (i < 2 ? lo : hi) * ((__int_as_float(sum[t][i]) - kMagicValue) * (i & 1 ? up.y : up.x));
-            }
+        for (int t = 0; t < NT; ++t) {
+          if (NT > 2 && t >= column_tiles) break;
+          const uint4 b = shared_w4[x_at[t] + u * 4];
+          const int magic[4] = {kMagic, kMagic, kMagic, kMagic};
+          int sum[4];
+          auto add = [&](int block) {
+            const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[t][i] += (i < 2 ? lo : hi)[block] * ((__int_as_float(sum[i]) - kMagicValue) * (i & 1 ? up.y : up.x));
+          };
+          mma(sum, f[0], b.x, b.y, magic);
+          if constexpr (HALVES) {
+            add(0);
+            mma(sum, f[1], b.z, b.w, magic);
+            add(1);
+          } else {
+            mma(sum, f[1], b.z, b.w, sum);
+            add(0);
           }
         }
         if (more) {
@@ -300,11 +307,13 @@ int shared_bytes(int nt, bool halves, int splits, int slots, int chunk, int cols
 
 template <int NT, bool HALVES, typename TSc>
 int launch(W4Params p, cudaStream_t s) {
-  constexpr int kWarps = kWarpsW4<NT>, kAhead = lvsa::kAhead<NT>;
+  constexpr int kWarps = kWarpsW4<NT>;
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
-  p.pass_rows = std::min(p.a.m, 8 * NT / kDigits);
-  const int passes = (p.a.m + p.pass_rows - 1) / p.pass_rows, ctas = std::max(1, sms / passes);
+  constexpr int kMost = 8 * NT / kDigits;
+  const int passes = (p.a.m + kMost - 1) / kMost;
+  p.pass_rows = (p.a.m + passes - 1) / passes;
+  const int ctas = std::max(1, sms / passes);
   // Rows of tiles of an SM; where they are fewer than the warps, more warps share one.
   const int share = (p.row_tiles + ctas - 1) / ctas;
   p.splits = std::max(1, std::min(kWarps / share, p.k_tiles));
@@ -332,15 +341,16 @@ int launch(W4Params p, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-template <typename TSc>
+template <bool HALVES, typename TSc>
 int launch_columns(const W4Params& p, cudaStream_t s) {
   const int64_t cols = static_cast<int64_t>(p.a.m) * kDigits;
-  if (p.a.group == 32) {
-    if (cols <= 8) return launch<1, true, TSc>(p, s);
-    return cols <= 16 ? launch<2, true, TSc>(p, s) : launch<4, true, TSc>(p, s);
-  }
-  if (cols <= 8) return launch<1, false, TSc>(p, s);
-  return cols <= 16 ? launch<2, false, TSc>(p, s) : launch<4, false, TSc>(p, s);
+  if (cols <= 8) return launch<1, HALVES, TSc>(p, s);
+  if (cols <= 16) return launch<2, HALVES, TSc>(p, s);
+  return cols <= 32 ? launch<4, HALVES, TSc>(p, s) : launch<8, HALVES, TSc>(p, s);
+}
+template <typename TSc>
+int launch_group(const W4Params& p, cudaStream_t s) {
+  return p.a.group == 32 ? launch_columns<true, TSc>(p, s) : launch_columns<false, TSc>(p, s);
 }
 
 }  // namespace
@@ -386,5 +396,5 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   p.x_vectors = vector_vector(Vector{a->x, a->ldx, 0, a->x_dtype}, 8);
   if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_columns<__nv_bfloat16>(p, s) : launch_columns<__half>(p, s);
+  return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_group<__nv_bfloat16>(p, s) : launch_group<__half>(p, s);
 }
