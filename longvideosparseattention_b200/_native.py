@@ -154,6 +154,8 @@ class LvsaError(RuntimeError):
 def load(path: str = LIB_PATH) -> ctypes.CDLL:
     """Load (once) and type the native library; raise if it is absent."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -180,17 +182,17 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         lib.lvsa_qk_prologue.restype = ctypes.c_int
         lib.lvsa_out_proj.argtypes = [ctypes.POINTER(LvsaOutProjArgs), _vp]
         lib.lvsa_out_proj.restype = ctypes.c_int
-        lib.lvsa_block_norm_fwd.argtypes = [ctypes.POINTER(LvsaBlockNorm), _vp]
+        lib.lvsa_block_norm_fwd.argtypes = [_vp, _vp]  # a structure by reference, or its bytes
         lib.lvsa_block_norm_fwd.restype = ctypes.c_int
-        lib.lvsa_block_norm_workspace.argtypes = [ctypes.POINTER(LvsaBlockNormGrad), ctypes.POINTER(_i64)]
+        lib.lvsa_block_norm_workspace.argtypes = [_vp, ctypes.POINTER(_i64)]
         lib.lvsa_block_norm_workspace.restype = ctypes.c_int
-        lib.lvsa_block_norm_bwd.argtypes = [ctypes.POINTER(LvsaBlockNormGrad), _vp]
+        lib.lvsa_block_norm_bwd.argtypes = [_vp, _vp]
         lib.lvsa_block_norm_bwd.restype = ctypes.c_int
         lib.lvsa_w4_bytes.argtypes = [_i32, _i32, ctypes.POINTER(_i64)]
         lib.lvsa_w4_bytes.restype = ctypes.c_int
         lib.lvsa_w4_pack.argtypes = [_vp, _i64, _i32, _i32, _vp, _vp]
         lib.lvsa_w4_pack.restype = ctypes.c_int
-        lib.lvsa_w4_linear.argtypes = [ctypes.POINTER(LvsaW4Linear), _vp]
+        lib.lvsa_w4_linear.argtypes = [_vp, _vp]
         lib.lvsa_w4_linear.restype = ctypes.c_int
         lib.lvsa_copy_segments.argtypes = [ctypes.POINTER(LvsaCopySegment), _i32, _i32, _vp]
         lib.lvsa_copy_segments.restype = ctypes.c_int

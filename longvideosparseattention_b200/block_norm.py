@@ -27,13 +27,14 @@ fp32 sums in a fixed order, so a step repeats bit for bit.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .block_sparse import _stream_ptr
+from ._launch import BLOCK_NORM, BLOCK_NORM_GRAD, launch
 
 _DT = {torch.bfloat16: N.LVSA_DTYPE_BF16, torch.float16: N.LVSA_DTYPE_F16, torch.float32: N.LVSA_DTYPE_F32}
 _KINDS = {"layer": N.LVSA_BLOCK_NORM_LAYER, "rms": N.LVSA_BLOCK_NORM_RMS}
@@ -70,151 +71,233 @@ def gate_residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Te
 
 
 # ------------------------------------------------------------------ arguments
+class _Form:
+    """What a call does, apart from its tensors."""
+    __slots__ = ("where", "join", "next", "post_kind", "post_eps", "kind", "eps", "alpha", "branch", "frames")
+
+
+_ABSENT = (0, 0, 0, 0, 0)
+_NO_ROWS = (0, 0, 0)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
-def _vectors(where: str, name: str, t: Optional[torch.Tensor], x: torch.Tensor) -> Optional[torch.Tensor]:
-    """A modulation tensor as [B or 1, F or 1, C]."""
-    if t is None:
-        return None
-    _same_device(where, name, t, x)
-    B, S, C = x.shape
-    v = t[None, None] if t.dim() == 1 else t[:, None] if t.dim() == 2 else t
-    if v.dim() != 3 or v.shape[2] != C or v.shape[0] not in (1, B):
-        raise ValueError(f"{where}: {name} must be [C], [B, C] or [B, F, C] for x {tuple(x.shape)}, got {tuple(t.shape)}")
-    return v if v.stride(2) == 1 or C == 1 else v.contiguous()
-
-
-def _channel(where: str, name: str, t: Optional[torch.Tensor], x: torch.Tensor) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    _same_device(where, name, t, x)
-    if t.dim() != 1 or t.shape[0] != x.shape[2]:
-        raise ValueError(f"{where}: {name} must be [{x.shape[2]}], got {tuple(t.shape)}")
-    return t if t.stride(0) == 1 or t.shape[0] == 1 else t.contiguous()
-
-
-def _same_device(where: str, name: str, t: torch.Tensor, x: torch.Tensor) -> None:
-    if t.device != x.device:
-        raise ValueError(f"{where}: {name} is on {t.device}, x on {x.device}")
-    if t.dtype not in _DT:
+def _typed(where: str, name: str, t: torch.Tensor, device: int) -> int:
+    if t.get_device() != device:
+        raise ValueError(f"{where}: {name} is on {t.device}, x on cuda:{device}")
+    code = _DT.get(t.dtype)
+    if code is None:
         raise TypeError(f"{where}: {name} must be bf16, fp16 or fp32, got {t.dtype}")
+    return code
+
+
+def _vectors(where: str, name: str, t: torch.Tensor, B: int, C: int, device: int) -> torch.Tensor:
+    """A modulation tensor, its channels contiguous, checked."""
+    _typed(where, name, t, device)
+    shape = t.shape
+    n = len(shape)
+    if not 1 <= n <= 3 or shape[-1] != C or (n > 1 and shape[0] != B and shape[0] != 1):
+        raise ValueError(f"{where}: {name} must be [C], [B, C] or [B, F, C] with B = {B} and C = {C}, got {tuple(shape)}")
+    return t if t.stride(-1) == 1 or C == 1 else t.contiguous()
+
+
+def _channel(where: str, name: str, t: torch.Tensor, C: int, device: int) -> torch.Tensor:
+    _typed(where, name, t, device)
+    if t.dim() != 1 or t.shape[0] != C:
+        raise ValueError(f"{where}: {name} must be [{C}], got {tuple(t.shape)}")
+    return t if C == 1 or t.stride(0) == 1 else t.contiguous()
 
 
 def _kind(where: str, name: str, kind: Optional[str]) -> int:
-    if kind is None:
-        return N.LVSA_BLOCK_NORM_NONE
-    try:
-        return _KINDS[kind]
-    except KeyError:
-        raise ValueError(f"{where}: {name} must be 'layer' or 'rms', got {kind!r}") from None
-
-
-class _Form:
-    """What a call does, apart from its tensors."""
-    __slots__ = ("where", "join", "next", "post_kind", "post_eps", "kind", "eps", "alpha", "branch", "frames")
+    code = _KINDS.get(kind)
+    if code is None:
+        raise ValueError(f"{where}: {name} must be 'layer' or 'rms', got {kind!r}")
+    return code
 
 
 def _run(where, x, y, gate, alpha, post_norm, post_weight, post_bias, post_eps, norm, weight, bias, scale, shift, eps,
          out_dtype):
     if not x.is_cuda:
         raise RuntimeError(f"{where} needs CUDA tensors (no CPU fallback)")
-    if x.dtype not in _DT:
-        raise TypeError(f"{where}: x must be bf16, fp16 or fp32, got {x.dtype}")
-    if x.dim() != 3 or not 1 <= x.shape[2] <= N.LVSA_BLOCK_NORM_MAX_WIDTH:
-        raise ValueError(f"{where}: x must be [B, S, C] with C of 1 to {N.LVSA_BLOCK_NORM_MAX_WIDTH}, got {tuple(x.shape)}")
+    dtype, shape, device = x.dtype, x.shape, x.get_device()
+    if dtype not in _DT:
+        raise TypeError(f"{where}: x must be bf16, fp16 or fp32, got {dtype}")
+    if len(shape) != 3 or not 1 <= shape[2] <= N.LVSA_BLOCK_NORM_MAX_WIDTH:
+        raise ValueError(f"{where}: x must be [B, S, C] with C of 1 to {N.LVSA_BLOCK_NORM_MAX_WIDTH}, got {tuple(shape)}")
+    B, S, C = shape
     form = _Form()
     form.where, form.join, form.next = where, y is not None, where != "gate_residual"
     form.alpha, form.eps, form.post_eps = float(alpha), float(eps), float(post_eps)
     if not (form.eps >= 0 and form.post_eps >= 0):
         raise ValueError(f"{where}: eps must not be negative")
-    form.kind, form.post_kind = _kind(where, "norm", norm), _kind(where, "post_norm", post_norm)
-    if form.next and not form.kind:
-        raise ValueError(f"{where}: norm must be 'layer' or 'rms'")
+    form.kind = _kind(where, "norm", norm) if form.next else 0
+    form.post_kind = _kind(where, "post_norm", post_norm) if post_norm is not None else 0
     if (bias is not None and norm != "layer") or (post_bias is not None and post_norm != "layer"):
         raise ValueError(f"{where}: only a layer norm has a bias")
     if post_weight is not None and not form.post_kind:
         raise ValueError(f"{where}: post_weight without post_norm")
     if form.join:
-        _same_device(where, "y", y, x)
-        if y.shape != x.shape:
-            raise ValueError(f"{where}: y {tuple(y.shape)} and x {tuple(x.shape)} differ")
+        _typed(where, "y", y, device)
+        if y.shape != shape:
+            raise ValueError(f"{where}: y {tuple(y.shape)} and x {tuple(shape)} differ")
         y = _rows(y)
         form.branch = y.dtype
+    elif where == "norm_modulate":
+        form.branch = dtype if out_dtype is None else out_dtype
     else:
-        if where != "norm_modulate":
-            raise ValueError(f"{where}: y is missing")
-        form.branch = out_dtype if out_dtype is not None else x.dtype
-    if form.branch != x.dtype and not (x.dtype == torch.float32 and form.branch in _DT):
-        raise TypeError(f"{where}: a {x.dtype} stream goes with {x.dtype} branches"
-                        f"{' or bf16 / fp16 ones' if x.dtype == torch.float32 else ''}, got {form.branch}")
+        raise ValueError(f"{where}: y is missing")
+    if form.branch != dtype and not (dtype == torch.float32 and form.branch in _DT):
+        raise TypeError(f"{where}: a {dtype} stream goes with {dtype} branches"
+                        f"{' or bf16 / fp16 ones' if dtype == torch.float32 else ''}, got {form.branch}")
     x = _rows(x)
-    gate, scale, shift = (_vectors(where, n, t, x) for n, t in (("gate", gate), ("scale", scale), ("shift", shift)))
-    weight, bias, post_weight, post_bias = (
-        _channel(where, n, t, x) for n, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight),
-                                              ("post_bias", post_bias)))
-    form.frames = max([v.shape[1] for v in (gate, scale, shift) if v is not None], default=1)
-    if form.frames < 1 or x.shape[1] % form.frames:
-        raise ValueError(f"{where}: {x.shape[1]} tokens do not divide into {form.frames} frames")
-    for name, v in (("gate", gate), ("scale", scale), ("shift", shift)):
-        if v is not None and v.shape[1] not in (1, form.frames):
-            raise ValueError(f"{where}: {name} has {v.shape[1]} frames, another vector {form.frames}")
+    frames = None
+    if gate is not None:
+        gate = _vectors(where, "gate", gate, B, C, device)
+        frames = gate.shape[1] if gate.dim() == 3 else 1
+    if scale is not None:
+        scale = _vectors(where, "scale", scale, B, C, device)
+        frames = _frames(where, "scale", scale, frames)
+    if shift is not None:
+        shift = _vectors(where, "shift", shift, B, C, device)
+        frames = _frames(where, "shift", shift, frames)
+    form.frames = 1 if frames is None else frames
+    if form.frames < 1 or S % form.frames:
+        raise ValueError(f"{where}: {S} tokens do not divide into {form.frames} frames")
+    if weight is not None:
+        weight = _channel(where, "weight", weight, C, device)
+    if bias is not None:
+        bias = _channel(where, "bias", bias, C, device)
+    if post_weight is not None:
+        post_weight = _channel(where, "post_weight", post_weight, C, device)
+    if post_bias is not None:
+        post_bias = _channel(where, "post_bias", post_bias, C, device)
     tensors = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        # A vector shared by sequences or frames: its gradient is summed in fp32 over them, then rounded once.
-        full = (x.shape[0], form.frames, x.shape[2])
-        gate, scale, shift = (v if v is None or not v.requires_grad or v.shape == full else v.float().expand(full)
-                              for v in (gate, scale, shift))
-        return _BlockNorm.apply(form, x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                full = (B, form.frames, C)
+                gate, scale, shift = (_full(v, full) for v in (gate, scale, shift))
+                return _BlockNorm.apply(form, x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
     return _forward(form, tensors, False)[:2]
 
 
+def _frames(where: str, name: str, v: torch.Tensor, frames: Optional[int]) -> int:
+    """The frames of v and of the vectors before it: those of any that has several."""
+    n = v.shape[1] if v.dim() == 3 else 1
+    if frames is None or frames == n or frames == 1:
+        return n
+    if n != 1:
+        raise ValueError(f"{where}: {name} has {n} frames, another vector {frames}")
+    return frames
+
+
+def _full(v: Optional[torch.Tensor], full: Tuple[int, int, int]) -> Optional[torch.Tensor]:
+    """A vector that needs a gradient as [B, F, C]: one that sequences or
+    frames share gets its gradient summed over them in fp32, rounded once."""
+    if v is None or not v.requires_grad or tuple(v.shape) == full:
+        return v
+    v = v[None, None] if v.dim() == 1 else v[:, None] if v.dim() == 2 else v
+    return v if tuple(v.shape) == full else v.float().expand(full)
+
+
 # ------------------------------------------------------------------- launches
-def _row_view(t: Optional[torch.Tensor]) -> N.LvsaRows:
+def _row_args(t: Optional[torch.Tensor]) -> Tuple[int, int, int]:
     if t is None:
-        return N.LvsaRows()
-    B, S, _ = t.shape
-    return N.LvsaRows(t.data_ptr(), t.stride(0) if B > 1 else 0, t.stride(1) if S > 1 else 0)
+        return _NO_ROWS
+    shape, stride = t.shape, t.stride()
+    return t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
 
 
-def _vector_view(t: Optional[torch.Tensor]) -> N.LvsaVectors:
+def _vector_args(t: Optional[torch.Tensor]) -> Tuple[int, int, int, int, int]:
     if t is None:
-        return N.LvsaVectors()
-    return N.LvsaVectors(t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0,
-                         _DT[t.dtype], 0)
+        return _ABSENT
+    shape, stride = t.shape, t.stride()
+    n = len(shape)
+    return (t.data_ptr(), stride[0] if n > 1 and shape[0] > 1 else 0, stride[1] if n == 3 and shape[1] > 1 else 0,
+            _DT[t.dtype], 0)
 
 
-def _norm_view(kind: int, eps: float, w: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> N.LvsaRowNorm:
-    return N.LvsaRowNorm(kind, eps, _DT[w.dtype] if w is not None else 0, _DT[b.dtype] if b is not None else 0,
-                         w.data_ptr() if w is not None else None, b.data_ptr() if b is not None else None)
+def _norm_args(kind: int, eps: float, w: Optional[torch.Tensor], b: Optional[torch.Tensor]):
+    return (kind, eps, 0 if w is None else _DT[w.dtype], 0 if b is None else _DT[b.dtype],
+            0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr())
 
 
-def _args(form: _Form, tensors, h, n, stats, post_stats) -> N.LvsaBlockNorm:
+def _args(form: _Form, tensors, h, n, stats, post_stats) -> tuple:
+    """LvsaBlockNorm's fields."""
     x, y, gate, scale, shift, weight, bias, post_weight, post_bias = tensors
     B, S, C = x.shape
-    return N.LvsaBlockNorm(_row_view(x), _row_view(y), _row_view(h), _row_view(n), _vector_view(gate),
-                           _vector_view(scale), _vector_view(shift),
-                           _norm_view(form.post_kind, form.post_eps, post_weight, post_bias),
-                           _norm_view(form.kind, form.eps, weight, bias), form.alpha, _DT[x.dtype], _DT[form.branch],
-                           B, S, form.frames, C, stats.data_ptr() if stats is not None else None,
-                           post_stats.data_ptr() if post_stats is not None else None)
+    return (*_row_args(x), *_row_args(y), *_row_args(h), *_row_args(n), *_vector_args(gate), *_vector_args(scale),
+            *_vector_args(shift), *_norm_args(form.post_kind, form.post_eps, post_weight, post_bias),
+            *_norm_args(form.kind, form.eps, weight, bias), form.alpha, _DT[x.dtype], _DT[form.branch], B, S,
+            form.frames, C, 0 if stats is None else stats.data_ptr(), 0 if post_stats is None else post_stats.data_ptr())
 
 
 def _forward(form: _Form, tensors, keep: bool):
     """(h or None, n or None, stats, post_stats); the statistics only where ``keep``."""
     x = tensors[0]
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if form.join else None
-    n = torch.empty(x.shape, dtype=form.branch, device=x.device) if form.next else None
-    rows = x.shape[0] * x.shape[1]
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if keep and form.next else None
-    post_stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if keep and form.post_kind else None
+    shape, device = x.shape, x.device
+    h = torch.empty(shape, dtype=x.dtype, device=device) if form.join else None
+    n = torch.empty(shape, dtype=form.branch, device=device) if form.next else None
+    rows = shape[0] * shape[1]
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=device) if keep and form.next else None
+    post_stats = torch.empty(rows, 2, dtype=torch.float32, device=device) if keep and form.post_kind else None
     if rows:
-        args = _args(form, tensors, h, n, stats, post_stats)
-        with torch.cuda.device(x.device):
-            st = N.load().lvsa_block_norm_fwd(ctypes.byref(args), _stream_ptr(x.device))
-        N.check(st, "lvsa_block_norm_fwd")
+        launch("lvsa_block_norm_fwd", BLOCK_NORM.pack(*_args(form, tensors, h, n, stats, post_stats)), x.get_device())
     return h, n, stats, post_stats
+
+
+@lru_cache(maxsize=256)
+def _workspace(stream: torch.dtype, branch: torch.dtype, B: int, S: int, frames: int, C: int, post: bool, join: bool,
+               totals: bool, device: int) -> int:
+    """Bytes that the backward of such a call needs, whatever its tensors."""
+    mark = N.LvsaRows(16, 0, 0)  # not read
+    g = N.LvsaBlockNormGrad()
+    g.f.x = g.f.n = mark
+    g.f.stats = g.f.post_stats = 16
+    g.f.next.kind = N.LVSA_BLOCK_NORM_LAYER
+    if join:
+        g.f.y = mark
+        g.f.post.kind = N.LVSA_BLOCK_NORM_LAYER if post else N.LVSA_BLOCK_NORM_NONE
+    g.f.stream_dtype, g.f.branch_dtype = _DT[stream], _DT[branch]
+    g.f.batch, g.f.seq, g.f.frames, g.f.width = B, S, frames, C
+    if totals:
+        g.f.next.weight = g.dweight = 16
+    size = ctypes.c_int64()
+    with torch.cuda.device(device):
+        N.check(N.load().lvsa_block_norm_workspace(ctypes.byref(g), ctypes.byref(size)), "lvsa_block_norm_workspace")
+    return size.value
+
+
+def _backward(ctx, dh, dn):
+    if dh is None and dn is None:
+        return (None,) * 10
+    form = ctx.form
+    saved = ctx.saved_tensors
+    tensors, stats, post_stats = saved[:9], saved[9], saved[10]
+    x = tensors[0]
+    B, S, C = x.shape
+    make = torch.empty_like if B * S else torch.zeros_like
+    grads = [make(t, memory_format=torch.contiguous_format) if wanted and t is not None else None
+             for t, wanted in zip(tensors, ctx.needs_input_grad[1:])]
+    if B * S:
+        dx, dy, dgate, dscale, dshift, dw, db, dpw, dpb = grads
+        totals = [0 if t is None else t.data_ptr() for t in (dw, db, dpw, dpb)]
+        device = x.get_device()
+        size = _workspace(x.dtype, form.branch, B, S, form.frames, C, form.post_kind != 0, form.join, any(totals), device)
+        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+        # n is set where there is a next norm, and not read.
+        args = BLOCK_NORM_GRAD.pack(
+            *_args(form, tensors, None, x if form.next else None, stats, post_stats),
+            *_row_args(None if dh is None else _rows(dh)), *_row_args(None if dn is None else _rows(dn)),
+            *_row_args(dx), *_row_args(dy), *_vector_args(dgate), *_vector_args(dscale), *_vector_args(dshift), *totals,
+            space.data_ptr(), size)
+        launch("lvsa_block_norm_bwd", args, device)
+    return (None, *grads)
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _BlockNorm(torch.autograd.Function):
@@ -227,33 +310,6 @@ class _BlockNorm(torch.autograd.Function):
         return h, n
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dn):
-        form = ctx.form
-        *tensors, stats, post_stats = ctx.saved_tensors
-        x, y, gate, scale, shift, weight, bias, post_weight, post_bias = tensors
-        need = ctx.needs_input_grad[1:]
-        if dh is None and dn is None:
-            return (None,) * 10
-        dh, dn = (None if d is None else _rows(d) for d in (dh, dn))
-        make = torch.empty if x.shape[0] * x.shape[1] else torch.zeros
-        grads = [make(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
-                 for t, wanted in zip(tensors, need)]
-        dx, dy, dgate, dscale, dshift, dw, db, dpw, dpb = grads
-        if x.shape[0] * x.shape[1]:
-            ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-            f = _args(form, tensors, None, None, stats, post_stats)
-            if form.next:  # says that there is a next norm; not read
-                f.n = _row_view(x)
-            args = N.LvsaBlockNormGrad(f, _row_view(dh), _row_view(dn), _row_view(dx), _row_view(dy),
-                                       _vector_view(dgate), _vector_view(dscale), _vector_view(dshift),
-                                       ptr(dw), ptr(db), ptr(dpw), ptr(dpb), None, 0)
-            lib, size = N.load(), ctypes.c_int64()
-            with torch.cuda.device(x.device):
-                N.check(lib.lvsa_block_norm_workspace(ctypes.byref(args), ctypes.byref(size)),
-                        "lvsa_block_norm_workspace")
-                space = torch.empty(size.value, dtype=torch.uint8, device=x.device)
-                args.workspace, args.workspace_bytes = space.data_ptr(), size.value
-                st = lib.lvsa_block_norm_bwd(ctypes.byref(args), _stream_ptr(x.device))
-            N.check(st, "lvsa_block_norm_bwd")
-        return (None, *grads)
+        # Under create_graph a second differentiation has to be refused.
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dh, dn)

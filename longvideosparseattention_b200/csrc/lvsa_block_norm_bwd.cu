@@ -417,7 +417,7 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   // A CTA ends with a piece of sums the size of some rows: not fewer than 8 rows each, unless SMs are left over.
   ctas = std::min(ctas, std::max<int64_t>(rows / 8, std::min<int64_t>(rows, device_sms())));
   if (ctas_only) {
-    *ctas_only = ctas;
+    *ctas_only = std::max(*ctas_only, ctas);
     return LVSA_OK;
   }
   float* space = static_cast<float*>(g.workspace);
@@ -441,9 +441,13 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   constexpr int VEC = kVec<TS>;
   const Vectors v(g.f);
   const int width = g.f.width;
-  if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
-      !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC))
+  if (ctas) {  // the workspace does not depend on the tensors' alignment
+    const int st = launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
+    if (st != LVSA_OK || width % VEC) return st;
+  } else if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
+      !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC)) {
     return launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
+  }
   if (width <= 8 * 256) return launch<TS, TB, FORM, VEC, 8 / VEC, 256, FORM ? 2 : 3>(g, v, ctas, s);
   if (width <= 8 * 640) return launch<TS, TB, FORM, VEC, 8 / VEC, 640, 1>(g, v, ctas, s);
   return launch<TS, TB, FORM, VEC, 16 / VEC, 512, 1>(g, v, ctas, s);

@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .block_sparse import _stream_ptr
+from ._launch import W4_LINEAR, launch
 
 _DT = {torch.bfloat16: N.LVSA_DTYPE_BF16, torch.float16: N.LVSA_DTYPE_F16, torch.float32: N.LVSA_DTYPE_F32}
 _ACT = {None: N.LVSA_W4_ACT_NONE, "silu": N.LVSA_W4_ACT_SILU}
@@ -66,7 +66,8 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, group: int) -> W4Weight:
     N.check(lib.lvsa_w4_bytes(n, k, ctypes.byref(size)), "lvsa_w4_bytes")
     tiles = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
     with torch.cuda.device(codes.device):
-        st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0), n, k, tiles.data_ptr(), _stream_ptr(codes.device))
+        st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0), n, k, tiles.data_ptr(),
+                              torch.cuda.current_stream().cuda_stream)
     N.check(st, "lvsa_w4_pack")
     # Two words a tile of 64 columns for group 32, one otherwise; a word has rows r and r + 8.
     rows, tile = -(-n // 16), max(1, 64 // group)
@@ -113,7 +114,7 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
         raise ValueError(f"linear_w4: activation must be None or 'silu', got {activation!r}")
     if x.dim() < 1 or x.shape[-1] != weight.k:
         raise ValueError(f"linear_w4: features of x {tuple(x.shape)} do not match weight [{weight.n}, {weight.k}]")
-    if weight.device != x.device or (bias is not None and bias.device != x.device):
+    if weight.tiles.get_device() != x.get_device() or (bias is not None and bias.get_device() != x.get_device()):
         raise ValueError("linear_w4: x, weight and bias must be on one device")
     if bias is not None and tuple(bias.shape) != (weight.n,):
         raise ValueError(f"linear_w4: bias must be [{weight.n}], got {tuple(bias.shape)}")
@@ -127,11 +128,9 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     m = rows.shape[0]
     out = torch.empty(m, weight.n, dtype=out_dtype, device=x.device)
     if m:
-        args = N.LvsaW4Linear(rows.data_ptr(), weight.tiles.data_ptr(), weight.scales.data_ptr(),
-                              bias.data_ptr() if bias is not None else None, out.data_ptr(), rows.stride(0), weight.n,
-                              m, weight.n, weight.k, weight.group, _DT[x.dtype], _DT[out_dtype],
-                              _DT[bias.dtype] if bias is not None else 0, _DT[weight.scales.dtype], _ACT[activation])
-        with torch.cuda.device(x.device):
-            st = N.load().lvsa_w4_linear(ctypes.byref(args), _stream_ptr(x.device))
-        N.check(st, "lvsa_w4_linear")
+        launch("lvsa_w4_linear", W4_LINEAR.pack(
+            rows.data_ptr(), weight.tiles.data_ptr(), weight.scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            out.data_ptr(), rows.stride(0), weight.n, m, weight.n, weight.k, weight.group, _DT[x.dtype],
+            _DT[out_dtype], 0 if bias is None else _DT[bias.dtype], _DT[weight.scales.dtype], _ACT[activation], 0),
+            x.get_device())
     return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.n)

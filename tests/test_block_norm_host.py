@@ -108,3 +108,20 @@ def test_cpu_tensors_are_refused():
     for call in (lambda: norm_modulate(x), lambda: gate_residual(x, x), lambda: gate_residual_norm(x, x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_packed_arguments_have_the_structures_layout():
+    """Fields packed as bytes fall where the C structures have them."""
+    from longvideosparseattention_b200 import _launch as L
+    for packer, struct in ((L.BLOCK_NORM, N.LvsaBlockNorm), (L.BLOCK_NORM_GRAD, N.LvsaBlockNormGrad),
+                           (L.W4_LINEAR, N.LvsaW4Linear)):
+        assert packer.size == ctypes.sizeof(struct)
+
+        def leaves(s):
+            for name, kind in s._fields_:
+                v = getattr(s, name)
+                yield from leaves(v) if isinstance(v, ctypes.Structure) else [0 if v is None else v]
+        n = len(packer.unpack(bytes(packer.size)))
+        values = list(range(1, n + 1))
+        got = list(leaves(struct.from_buffer_copy(packer.pack(*values))))
+        assert got == values[:len(got)] and n - len(got) in (0, 1)
