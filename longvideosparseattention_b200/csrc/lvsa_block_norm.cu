@@ -231,8 +231,8 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
   const int shared = vectors_held * shared_pitch(a.width) * static_cast<int>(sizeof(float)) +
                      (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + (JOIN ? sizeof(TB) : 0)) : 0);
   auto kern = block_norm_fwd_kernel<TS, TB, FORM, VEC, K>;
-  static std::atomic<uint64_t> last{0};
-  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last);
+  static std::atomic<uint64_t> done{0}, last{0};
+  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
   const FwdParams p{a.x, a.y, a.h, a.n, v, FastDiv(a.seq), FastDiv(a.seq / a.frames), static_cast<uint32_t>(rows),
                     static_cast<uint32_t>(a.frames), a.width, warps, vectors_held, a.next.kind, a.post.kind, a.residual_scale,

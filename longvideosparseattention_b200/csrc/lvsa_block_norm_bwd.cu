@@ -199,6 +199,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
     const float2 st = st_ahead, ps = ps_ahead;
     // d: gradient of z, yh: yhat.  Columns outside the row stay zero.
     float d[K][VEC], yh[JOIN ? K : 1][VEC], zh[K][VEC], v[K][VEC];
+    const float mr = st.x * st.y, pmr = ps.x * ps.y;
     float s = 0.f, sz = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         if (more) take(hr, hs, k, d[k]);
         if constexpr (POST) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) yh[k][e] = (yh[k][e] - ps.x) * ps.y;
+          for (int e = 0; e < VEC; ++e) yh[k][e] = yh[k][e] * ps.y - pmr;
         }
       }
       if (!next) continue;
@@ -233,7 +234,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       A.get(32 * k, q);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        zh[k][e] = (zh[k][e] - st.x) * st.y;
+        zh[k][e] = zh[k][e] * st.y - mr;
         P[k][e] += v[k][e] * zh[k][e];
         Q[k][e] += v[k][e];
         v[k][e] *= q[e];
@@ -244,12 +245,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
     if (RING && row + 1 < r1) fetch();
     if (next) {
       const float2 m = team.sum2(s, sz);
-      const float m0 = a.next.kind == LVSA_BLOCK_NORM_LAYER ? m.x * inv : 0.f, m1 = m.y * inv;
+      const float m0 = a.next.kind == LVSA_BLOCK_NORM_LAYER ? st.y * (m.x * inv) : 0.f, m1 = st.y * (m.y * inv);
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (col.in(k)) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[k][e] += st.y * ((v[k][e] - m0) - zh[k][e] * m1);
+          for (int e = 0; e < VEC; ++e) d[k][e] = (d[k][e] - m0) + (v[k][e] * st.y - zh[k][e] * m1);
         }
     }
     if (g.dx.ptr) {
@@ -286,15 +287,15 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         float m0 = 0.f, m1 = 0.f;
         if constexpr (POST) {
           const float2 m = team.sum2(s, sy);
-          m0 = a.post.kind == LVSA_BLOCK_NORM_LAYER ? m.x * inv : 0.f;
-          m1 = m.y * inv;
+          m0 = a.post.kind == LVSA_BLOCK_NORM_LAYER ? ps.y * (m.x * inv) : 0.f;
+          m1 = ps.y * (m.y * inv);
         }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           if (!col.in(k)) continue;
           if constexpr (POST) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) d[k][e] = ps.y * ((d[k][e] - m0) - yh[k][e] * m1);
+            for (int e = 0; e < VEC; ++e) d[k][e] = (d[k][e] * ps.y - m0) - yh[k][e] * m1;
           }
           PB::store(dy + k * col.kStep, d[k]);
         }
@@ -408,11 +409,11 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   auto kern = block_norm_bwd_kernel<TS, TB, FORM, VEC, K, THREADS, CTAS>;
   const int vectors = (g.f.width + VEC - 1) / VEC;
   const int threads = ((vectors + K - 1) / K + 31) / 32 * 32;
-  static std::atomic<uint64_t> last{0};
+  static std::atomic<uint64_t> done{0}, last{0};
   const int64_t rows = static_cast<int64_t>(g.f.batch) * g.f.seq;
   const int shared = (FORM + 1) * shared_pitch(g.f.width) * static_cast<int>(sizeof(float)) +
                      (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
-  int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, last);
+  int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
   // A CTA ends with a piece of sums the size of some rows: not fewer than 8 rows each, unless SMs are left over.
   ctas = std::min(ctas, std::max<int64_t>(rows / 8, std::min<int64_t>(rows, device_sms())));

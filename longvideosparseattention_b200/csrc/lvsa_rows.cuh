@@ -146,61 +146,67 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 // Two sums at once: after the first exchange the lower lanes carry a, the
-// upper ones b, so that the pair costs six exchanges rather than ten.
-__device__ __forceinline__ float2 warp_sum2(float a, float b) {
+// upper ones b.  Leaves a in lanes 0 .. 15, b in the others.
+__device__ __forceinline__ float warp_sum2(float a, float b) {
   const bool up = threadIdx.x & 16;
   float mine = up ? b : a;
   mine += __shfl_xor_sync(0xffffffffu, up ? a : b, 16);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  const float other = __shfl_xor_sync(0xffffffffu, mine, 16);
-  return up ? make_float2(other, mine) : make_float2(mine, other);
+  return mine;
 }
 
 constexpr int kMaxWarps = 32;  // of a CTA
 
-// The warps that hold one row: `count` of them, `slots` [2][count] of their
-// own in shared memory, a hardware barrier of their own.  One barrier a sum:
-// the slots alternate, and a thread that writes a slot again has passed the
-// barrier of the sum between, which every reader of the slot has reached
+// The warps that hold one row: `count` of them, `slots` [2][count] pairs of
+// their own in shared memory, a hardware barrier of their own.  One barrier a
+// sum: the slots alternate, and a thread that writes a slot again has passed
+// the barrier of the sum between, which every reader of the slot has reached
 // after reading it.
 struct Team {
-  float2* slots;
-  int count, warp, lane, barrier, turn;
+  float* slots;
+  int count, round, warp, lane, barrier, turn;  // round: the power of two at or above count
 
   __device__ __forceinline__ Team(float2* all, int warps_a_team)
       : count(warps_a_team), lane(threadIdx.x & 31), turn(0) {
     const int w = threadIdx.x >> 5, team = w / warps_a_team;
     warp = w - team * warps_a_team;
-    slots = all + 2 * team * warps_a_team;
+    slots = reinterpret_cast<float*>(all + 2 * team * warps_a_team);
     barrier = team + 1;
+    round = count > 1 ? 1 << (32 - __clz(count - 1)) : 1;
   }
-  // Every warp's pair, after the barrier.
-  __device__ __forceinline__ const float2* exchange(float2 mine) {
-    float2* s = slots + turn * count;
+  // Where this turn's pairs go: [2 warp], [2 warp + 1].
+  __device__ __forceinline__ float* turn_slots() {
+    float* s = slots + turn * 2 * count;
     turn ^= 1;
-    if (lane == 0) s[warp] = mine;
-    if (count * 32 == blockDim.x) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
     return s;
   }
-  // Few warps are added one after another by every thread, many by exchanges.
-  __device__ __forceinline__ float2 sum2(float a, float b) {
-    float2 v = warp_sum2(a, b);
-    if (count == 1) return v;
-    const float2* s = exchange(v);
-    if (count <= kFew) {
-      v = s[0];
-      for (int w = 1; w < count; ++w) {
-        v.x += s[w].x;
-        v.y += s[w].y;
-      }
-      return v;
-    }
-    v = lane < count ? s[lane] : make_float2(0.f, 0.f);
-    return warp_sum2(v.x, v.y);
+  __device__ __forceinline__ void sync() {
+    if (count * 32 == blockDim.x) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
   }
-  static constexpr int kFew = 6;
+  // Over the team, of what lane l holds of warp l modulo `round`.
+  __device__ __forceinline__ float over_warps(float v) {
+    for (int o = 1; o < round; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  __device__ __forceinline__ float2 sum2(float a, float b) {
+    float v = warp_sum2(a, b);
+    if (count > 1) {
+      float* s = turn_slots();
+      if ((lane & 15) == 0) s[2 * warp + (lane >> 4)] = v;
+      sync();
+      // Lane l takes float l of the pairs and adds up those of its parity.
+      const int at = lane & (2 * round - 1);
+      v = at < 2 * count ? s[at] : 0.f;
+      if (count > 16) v += lane + 32 < 2 * count ? s[lane + 32] : 0.f;
+      for (int o = 2; o < min(2 * round, 32); o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      const float other = __shfl_xor_sync(0xffffffffu, v, 1);
+      return lane & 1 ? make_float2(other, v) : make_float2(v, other);
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+    return lane & 16 ? make_float2(other, v) : make_float2(v, other);
+  }
 };
 
 // Columns of one thread: a warp holds K x 32 vectors of VEC side by side, the
@@ -296,13 +302,11 @@ __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Colu
       }
     q = warp_sum(q);
     if (team.count > 1) {
-      const float2* g = team.exchange(make_float2(q, 0.f));
-      if (team.count <= Team::kFew) {
-        q = g[0].x;
-        for (int w = 1; w < team.count; ++w) q += g[w].x;
-      } else {
-        q = warp_sum(team.lane < team.count ? g[team.lane].x : 0.f);
-      }
+      float* g = team.turn_slots();
+      if (team.lane == 0) g[2 * team.warp] = q;
+      team.sync();
+      const int w = team.lane & (team.round - 1);
+      q = team.over_warps(w < team.count ? g[2 * w] : 0.f);
     }
     return make_float2(0.f, rsqrtf(q * held.inv_row + eps));
   }
@@ -326,23 +330,19 @@ __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Colu
     }
   q = warp_sum(q);
   if (team.count > 1) {
-    const float2* g = team.exchange(make_float2(mean, q));
-    if (team.count <= Team::kFew) {
-      mean = 0.f;
-      for (int w = 0; w < team.count; ++w) mean += held.counts[w] * g[w].x;
-      mean *= held.inv_row;
-      q = 0.f;
-      for (int w = 0; w < team.count; ++w) {
-        const float d = g[w].x - mean;
-        q += g[w].y + held.counts[w] * d * d;
-      }
-    } else {
-      const float2 m = team.lane < team.count ? g[team.lane] : make_float2(0.f, 0.f);
-      const float n = team.lane < team.count ? held.counts[team.lane] : 0.f;
-      mean = warp_sum(n * m.x) * held.inv_row;
-      const float d = m.x - mean;
-      q = warp_sum(m.y + n * d * d);
+    float* g = team.turn_slots();
+    if (team.lane == 0) {
+      g[2 * team.warp] = mean;
+      g[2 * team.warp + 1] = q;
     }
+    team.sync();
+    const int w = team.lane & (team.round - 1);
+    const bool real = w < team.count;
+    const float m = real ? g[2 * w] : 0.f, n = real ? held.counts[w] : 0.f;
+    q = real ? g[2 * w + 1] : 0.f;
+    mean = team.over_warps(n * m) * held.inv_row;
+    const float d = m - mean;
+    q = team.over_warps(q + n * d * d);
   }
   return make_float2(mean, rsqrtf(q * held.inv_row + eps));
 }
@@ -397,13 +397,27 @@ inline int device_sms() {
   }
   return n;
 }
+// Allows `kern` the most shared memory that a CTA may have, once a device:
+// `done` keeps a bit for each.
+inline bool allow_shared(const void* kern, std::atomic<uint64_t>& done) {
+  int dev = 0, most = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return true;
+  cudaFuncAttributes has;
+  if (cudaFuncGetAttributes(&has, kern) != cudaSuccess ||
+      cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess ||
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           most - static_cast<int>(has.sharedSizeBytes)) != cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 // CTAs of `kern` that fit the device at once.  `last` keeps the answer for the
-// last shape asked for (every device of a process is the same chip; the
-// permission for more than 48 KB of shared memory is each device's own).
-inline int64_t resident_ctas(const void* kern, int threads, int shared, std::atomic<uint64_t>& last) {
-  if (shared > 40 * 1024 &&  // with what a kernel declares itself, 48 KB need no permission
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess)
-    return 0;
+// last shape asked for (every device of a process is the same chip).
+inline int64_t resident_ctas(const void* kern, int threads, int shared, std::atomic<uint64_t>& done,
+                             std::atomic<uint64_t>& last) {
+  if (!allow_shared(kern, done)) return 0;
   const uint64_t shape = static_cast<uint64_t>(shared) << 32 | static_cast<uint64_t>(threads) << 16;
   const uint64_t seen = last.load(std::memory_order_relaxed);
   if (seen >> 16 == shape >> 16 && (seen & 0xffff)) return seen & 0xffff;

@@ -25,6 +25,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 
 #include "lvsa_rows.cuh"
@@ -336,7 +337,8 @@ int launch(W4Params p, cudaStream_t s) {
   p.pitch = column_pitch(p.splits * p.chunk);
   auto kern = w4_linear_kernel<NT, HALVES, TSc>;
   const int shared = shared_of();
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, shared) != cudaSuccess) return LVSA_ERR_CUDA;
+  static std::atomic<uint64_t> done{0};
+  if (!allow_shared(reinterpret_cast<const void*>(kern), done)) return LVSA_ERR_CUDA;
   kern<<<dim3(std::min(p.row_tiles, ctas), passes), 32 * kWarps, shared, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
