@@ -165,17 +165,13 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
             float branch[VEC], g[VEC];
             take_x(k, z[k]);
             take_y(k, branch);
-            if constexpr (POST) {
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) branch[e] = (branch[e] - st.x) * st.y;
-            }
+            if constexpr (POST) vfma(branch, branch, st.y, -st.x * st.y);
             vkG1.get(32 * k, g);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) z[k][e] = p.alpha * z[k][e] + branch[e] * g[e];
+            vmul(z[k], z[k], p.alpha);
+            vfma(z[k], branch, g, z[k]);
             if (g0) {
               vkG0.get(32 * k, g);
-#pragma unroll
-              for (int e = 0; e < VEC; ++e) z[k][e] += g[e];
+              vadd(z[k], z[k], g);
             }
           }
       } else {
@@ -200,8 +196,8 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
             float A[VEC], B[VEC];
             vkA.get(32 * k, A);
             vkB.get(32 * k, B);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) A[e] = (z[k][e] * st.y - mr) * A[e] + B[e];
+            vfma(z[k], z[k], st.y, -mr);
+            vfma(A, z[k], A, B);
             Pack<TB, VEC>::store(n + k * col.kStep, A);
           }
         n += teams * p.n.stride_t;
@@ -217,10 +213,7 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
   const int vectors = (a.width + VEC - 1) / VEC;
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
-  // Warps a row: as few as hold it, or one access a thread where the rows do
-  // not fill the device anyway and a row's latency is the time.
-  int warps = (vectors + 32 * K - 1) / (32 * K);
-  if (rows <= 4 * sms) warps = std::max(warps, std::min(16, (vectors + 31) / 32));
+  const int warps = (vectors + 32 * K - 1) / (32 * K);
   // Teams a CTA: one CTA fills an SM, its vectors held once; fewer while SMs
   // are left over or a group has few rows to share its vectors.
   int teams = std::max(1, std::min(kThreads<VEC, FORM> / (32 * warps), warps == 1 ? 32 : 15));
@@ -248,10 +241,13 @@ int launch_width(const LvsaBlockNorm& a, cudaStream_t s) {
   // Widths, strides or pointers that 16-byte accesses do not fit go value by value.
   if (a.width % VEC == 0 && rows_vector<TS, VEC>(a.x) && rows_vector<TB, VEC>(a.y) && rows_vector<TS, VEC>(a.h) &&
       rows_vector<TB, VEC>(a.n) && v.aligned(VEC)) {
-    // The fewest warps of kElems values a thread, then the fewest values.
+    // The fewest warps of kElems values a thread, then the fewest values; half
+    // of kElems where the rows do not fill the device and a row's latency is
+    // the time (2 x 77 rows of 2048: 4.5 us with 32 values, FEW_US with 16).
     const int vectors = a.width / VEC, warps = (vectors * VEC + 32 * kElems - 1) / (32 * kElems);
-    const int k = (vectors + 32 * warps - 1) / (32 * warps);
     constexpr int kMost = kElems / VEC;
+    const bool few = static_cast<int64_t>(a.batch) * a.seq <= 4 * device_sms();
+    const int k = few ? 1 : (vectors + 32 * warps - 1) / (32 * warps);
     return k > kMost * 3 / 4 ? launch<TS, TB, FORM, VEC, kMost>(a, v, s)
            : k > kMost / 2   ? launch<TS, TB, FORM, VEC, kMost * 3 / 4>(a, v, s)
                              : launch<TS, TB, FORM, VEC, kMost / 2>(a, v, s);

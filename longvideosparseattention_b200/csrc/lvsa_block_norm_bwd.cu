@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
     // d: gradient of z, yh: yhat.  Columns outside the row stay zero.
     float d[K][VEC], yh[JOIN ? K : 1][VEC], zh[K][VEC], v[K][VEC];
     const float mr = st.x * st.y, pmr = ps.x * ps.y;
-    float s = 0.f, sz = 0.f;
+    float2 s = make_float2(0.f, 0.f), sz = s;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -212,10 +212,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       if constexpr (JOIN) {
         take(yr, ys, k, yh[k]);
         if (more) take(hr, hs, k, d[k]);
-        if constexpr (POST) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) yh[k][e] = yh[k][e] * ps.y - pmr;
-        }
+        if constexpr (POST) vfma(yh[k], yh[k], ps.y, -pmr);
       }
       if (!next) continue;
       take(xr, xs, k, zh[k]);
@@ -223,70 +220,66 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       float q[VEC];
       if constexpr (JOIN) {
         G1.get(32 * k, q);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zh[k][e] = a.residual_scale * zh[k][e] + yh[k][e] * q[e];
+        vmul(q, yh[k], q);
+        vfma(zh[k], zh[k], a.residual_scale, q);
       }
       if constexpr (POST) {
         G0.get(32 * k, q);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) zh[k][e] += q[e];
+        vadd(zh[k], zh[k], q);
       }
       A.get(32 * k, q);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        zh[k][e] = zh[k][e] * st.y - mr;
-        P[k][e] += v[k][e] * zh[k][e];
-        Q[k][e] += v[k][e];
-        v[k][e] *= q[e];
-        s += v[k][e];
-        sz += v[k][e] * zh[k][e];
-      }
+      vfma(zh[k], zh[k], st.y, -mr);
+      vfma(P[k], v[k], zh[k], P[k]);
+      vadd(Q[k], Q[k], v[k]);
+      vmul(v[k], v[k], q);
+      sum_on(s, v[k]);
+      sum_on(sz, v[k], zh[k]);
     }
     if (RING && row + 1 < r1) fetch();
     if (next) {
-      const float2 m = team.sum2(s, sz);
+      const float2 m = team.sum2(s.x + s.y, sz.x + sz.y);
       const float m0 = a.next.kind == LVSA_BLOCK_NORM_LAYER ? st.y * (m.x * inv) : 0.f, m1 = st.y * (m.y * inv);
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (col.in(k)) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) d[k][e] = (d[k][e] - m0) + (v[k][e] * st.y - zh[k][e] * m1);
+          vadd(d[k], d[k], -m0);
+          vfma(d[k], v[k], st.y, d[k]);
+          vfma(d[k], zh[k], -m1, d[k]);
         }
     }
     if (g.dx.ptr) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!col.in(k)) continue;
-        float o[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = JOIN ? a.residual_scale * d[k][e] : d[k][e];
-        PS::store(dx + k * col.kStep, o);
+        if constexpr (JOIN) {
+          float o[VEC];
+          vmul(o, d[k], a.residual_scale);
+          PS::store(dx + k * col.kStep, o);
+        } else {
+          PS::store(dx + k * col.kStep, d[k]);
+        }
       }
       dx += g.dx.stride_t;
     }
     if constexpr (JOIN) {
-      float sy = 0.f;
-      s = 0.f;
+      s = sz = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         if (!col.in(k)) continue;
         float q[VEC];
         G1.get(32 * k, q);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          P2[k][e] += d[k][e] * yh[k][e];
-          if constexpr (POST) Q2[k][e] += d[k][e];
-          d[k][e] *= q[e];
-          if constexpr (POST) {
-            s += d[k][e];
-            sy += d[k][e] * yh[k][e];
-          }
+        vfma(P2[k], d[k], yh[k], P2[k]);
+        if constexpr (POST) vadd(Q2[k], Q2[k], d[k]);
+        vmul(d[k], d[k], q);
+        if constexpr (POST) {
+          sum_on(s, d[k]);
+          sum_on(sz, d[k], yh[k]);
         }
       }
       if (g.dy.ptr) {
         float m0 = 0.f, m1 = 0.f;
         if constexpr (POST) {
-          const float2 m = team.sum2(s, sy);
+          const float2 m = team.sum2(s.x + s.y, sz.x + sz.y);
           m0 = a.post.kind == LVSA_BLOCK_NORM_LAYER ? ps.y * (m.x * inv) : 0.f;
           m1 = ps.y * (m.y * inv);
         }
@@ -294,8 +287,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         for (int k = 0; k < K; ++k) {
           if (!col.in(k)) continue;
           if constexpr (POST) {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) d[k][e] = (d[k][e] * ps.y - m0) - yh[k][e] * m1;
+            vfma(d[k], d[k], ps.y, -m0);
+            vfma(d[k], yh[k], -m1, d[k]);
           }
           PB::store(dy + k * col.kStep, d[k]);
         }
@@ -443,12 +436,13 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   const Vectors v(g.f);
   const int width = g.f.width;
   if (ctas) {  // the workspace does not depend on the tensors' alignment
-    const int st = launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
+    const int st = width <= 8 * 384 ? launch<TS, TB, FORM, 1, 8, 384, 1>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
     if (st != LVSA_OK || width % VEC) return st;
   } else if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
       !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC)) {
-    return launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
+    return width <= 8 * 384 ? launch<TS, TB, FORM, 1, 8, 384, 1>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
   }
+  if (width <= 8 * 192) return launch<TS, TB, FORM, VEC, 8 / VEC, 192, FORM ? 3 : 4>(g, v, ctas, s);
   if (width <= 8 * 256) return launch<TS, TB, FORM, VEC, 8 / VEC, 256, FORM ? 2 : 3>(g, v, ctas, s);
   if (width <= 8 * 640) return launch<TS, TB, FORM, VEC, 8 / VEC, 640, 1>(g, v, ctas, s);
   return launch<TS, TB, FORM, VEC, 16 / VEC, 512, 1>(g, v, ctas, s);

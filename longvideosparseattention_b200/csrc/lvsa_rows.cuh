@@ -70,6 +70,101 @@ struct Pack {
   }
 };
 
+// Arithmetic on N values at a time, two an instruction (f32x2): these kernels
+// are close to bound by the instructions they issue.  An operand may be one
+// number for all.
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 p, q, r, s;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
+      "fma.rn.f32x2 s, p, q, r;\n\tmov.b64 {%0, %1}, s;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 p, q, s;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 s, p, q;\n\tmov.b64 {%0, %1}, s;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 p, q, s;\n\t"
+      "mov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tadd.rn.f32x2 s, p, q;\n\tmov.b64 {%0, %1}, s;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+template <int N>
+__device__ __forceinline__ float2 pair_of(const float (&a)[N], int i) { return make_float2(a[i], a[i + 1]); }
+__device__ __forceinline__ float2 pair_of(float a, int) { return make_float2(a, a); }
+template <int N>
+__device__ __forceinline__ float one_of(const float (&a)[N]) { return a[0]; }
+__device__ __forceinline__ float one_of(float a) { return a; }
+
+// d = a b + c, d = a b, d = a + b.
+template <int N, typename A, typename B, typename C>
+__device__ __forceinline__ void vfma(float (&d)[N], const A& a, const B& b, const C& c) {
+  if constexpr (N == 1) {
+    d[0] = fmaf(one_of(a), one_of(b), one_of(c));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = fma_pair(pair_of(a, i), pair_of(b, i), pair_of(c, i));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  }
+}
+template <int N, typename A, typename B>
+__device__ __forceinline__ void vmul(float (&d)[N], const A& a, const B& b) {
+  if constexpr (N == 1) {
+    d[0] = one_of(a) * one_of(b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = mul_pair(pair_of(a, i), pair_of(b, i));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  }
+}
+template <int N, typename A, typename B>
+__device__ __forceinline__ void vadd(float (&d)[N], const A& a, const B& b) {
+  if constexpr (N == 1) {
+    d[0] = one_of(a) + one_of(b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 r = add_pair(pair_of(a, i), pair_of(b, i));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  }
+}
+// s += a, s += a b, into two running sums (one where N is 1).
+template <int N>
+__device__ __forceinline__ void sum_on(float2& s, const float (&a)[N]) {
+  if constexpr (N == 1) {
+    s.x += a[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) s = add_pair(s, pair_of(a, i));
+  }
+}
+template <int N>
+__device__ __forceinline__ void sum_on(float2& s, const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N == 1) {
+    s.x = fmaf(a[0], b[0], s.x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) s = fma_pair(pair_of(a, i), pair_of(b, i), s);
+  }
+}
+
 // A vector of the channels whose type is known at run time (modulation, norm
 // parameters): element strides between sequences and frames, ptr NULL: absent.
 struct Vector {
@@ -292,14 +387,12 @@ struct Held {
 template <int VEC, int K>
 __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Columns<VEC, K>& col, int kind, float eps,
                                             const Held& held, Team& team) {
+  float2 run = make_float2(0.f, 0.f);
   if (kind == LVSA_BLOCK_NORM_RMS) {
-    float q = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (col.in(k)) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) q += z[k][e] * z[k][e];
-      }
+      if (col.in(k)) sum_on(run, z[k], z[k]);
+    float q = run.x + run.y;
     q = warp_sum(q);
     if (team.count > 1) {
       float* g = team.turn_slots();
@@ -310,24 +403,19 @@ __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Colu
     }
     return make_float2(0.f, rsqrtf(q * held.inv_row + eps));
   }
-  float mean = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    if (col.in(k)) sum_on(run, z[k]);
+  float mean = warp_sum(run.x + run.y) * held.inv_mine;
+  run = make_float2(0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < K; ++k)
     if (col.in(k)) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) mean += z[k][e];
+      float d[VEC];
+      vadd(d, z[k], -mean);
+      sum_on(run, d, d);
     }
-  mean = warp_sum(mean) * held.inv_mine;
-  float q = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if (col.in(k)) {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = z[k][e] - mean;
-        q += d * d;
-      }
-    }
+  float q = run.x + run.y;
   q = warp_sum(q);
   if (team.count > 1) {
     float* g = team.turn_slots();
