@@ -58,6 +58,10 @@ __device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t 
   }
 }
 
+// Rows on their way into shared memory.
+template <int FORM, int COLUMNS>
+constexpr int kDepth = FORM == 2 || COLUMNS > 8 ? 1 : 2;
+
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
 template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __grid_constant__ BwdParams p) {
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
   const float inv = 1.f / static_cast<float>(a.width);
   const uint32_t r0 = static_cast<uint32_t>(first_row(p.rows, blockIdx.x, p.ctas));
   const uint32_t r1 = static_cast<uint32_t>(first_row(p.rows, blockIdx.x + 1, p.ctas));
-  const bool next = g.dn.ptr, more = JOIN && g.dh.ptr;
+  const bool next = g.dn.ptr, more = JOIN && g.dh.ptr, bias = POST && a.post.bias;
 
   // A, G1 and G0 of this thread's columns, and its part of the next row: read
   // and written by their own thread alone, so that no barrier is due.
@@ -85,13 +89,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
   typename PS::R* const hs = xs + K * blockDim.x;
   typename PB::R* const ns = reinterpret_cast<typename PB::R*>(hs - threadIdx.x + (JOIN ? K * blockDim.x : 0)) + threadIdx.x;
   typename PB::R* const ys = ns + K * blockDim.x;
+  // Two rows on their way, in turn (77910 x 2048 with a join 370 us with one
+  // row, 325 with two; with a norm of the branch 444 and 510 at 17550 x 5120).
+  constexpr int DEPTH = kDepth<FORM, VEC * K>;
+  const int row_bytes = K * blockDim.x * static_cast<int>(sizeof(xs[0]) + sizeof(ns[0])) * (JOIN ? 2 : 1);
+  int put_at = 0, take_at = 0;  // bytes to the row to fetch, and to take
+  auto slot_of = [&](auto* slot, int k, int at) {
+    return reinterpret_cast<decltype(slot)>(reinterpret_cast<char*>(slot + k * blockDim.x) + at);
+  };
   PS xr[RING ? 1 : K], hr[RING || !JOIN ? 1 : K];  // the row itself where nothing can be copied ahead
   PB nr[RING ? 1 : K], yr[RING || !JOIN ? 1 : K];
 
   const TS *x = nullptr, *dh = nullptr;
   const TB *y = nullptr, *dn = nullptr;
   uint32_t ahead = r0, ahead_end = r0;  // the row that fetch() takes, and where its sequence ends
-  float2 st_ahead = make_float2(0.f, 1.f), ps_ahead = st_ahead;
   auto fetch = [&]() {
     if (ahead == ahead_end) {
       const uint32_t fb = p.by_seq.div(ahead);
@@ -104,19 +115,17 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         dh = static_cast<const TS*>(g.dh.ptr) + fb * g.dh.stride_b + t * g.dh.stride_t + col.first;
       }
     }
-    if (next) st_ahead = __ldg(reinterpret_cast<const float2*>(a.stats) + ahead);
-    if constexpr (POST) ps_ahead = __ldg(reinterpret_cast<const float2*>(a.post_stats) + ahead);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!col.in(k)) continue;
       if constexpr (RING) {
         if (next) {
-          copy_async<sizeof(xs[0])>(xs + k * blockDim.x, x + k * col.kStep);
-          copy_async<sizeof(ns[0])>(ns + k * blockDim.x, dn + k * col.kStep);
+          copy_async<sizeof(xs[0])>(slot_of(xs, k, put_at), x + k * col.kStep);
+          copy_async<sizeof(ns[0])>(slot_of(ns, k, put_at), dn + k * col.kStep);
         }
         if constexpr (JOIN) {
-          copy_async<sizeof(ys[0])>(ys + k * blockDim.x, y + k * col.kStep);
-          if (more) copy_async<sizeof(hs[0])>(hs + k * blockDim.x, dh + k * col.kStep);
+          copy_async<sizeof(ys[0])>(slot_of(ys, k, put_at), y + k * col.kStep);
+          if (more) copy_async<sizeof(hs[0])>(slot_of(hs, k, put_at), dh + k * col.kStep);
         }
       } else {
         if (next) {
@@ -130,6 +139,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       }
     }
     ++ahead;
+    if constexpr (DEPTH == 2) put_at = row_bytes - put_at;
     x += a.x.stride_t;
     dn += g.dn.stride_t;
     if constexpr (JOIN) {
@@ -137,8 +147,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       dh += g.dh.stride_t;
     }
   };
-  auto take = [&](auto& row, const auto* slot, int k, float(&f)[VEC]) {
-    if constexpr (RING) row[0].u = slot[k * blockDim.x];
+  auto take = [&](auto& row, auto* slot, int k, float(&f)[VEC]) {
+    if constexpr (RING) row[0].u = *slot_of(slot, k, take_at);
     row[RING ? 0 : k].get(f);
   };
 
@@ -148,7 +158,22 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
   int64_t b = 0, f = 0;
   TS* dx = nullptr;
   TB* dy = nullptr;
-  if (RING) fetch();
+  // A group of copies a row, empty past the last.
+  auto fetch_group = [&]() {
+    if (ahead < r1) fetch();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (RING) {
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i) fetch_group();
+  }
+  float2 st_ahead = make_float2(0.f, 1.f), ps_ahead = st_ahead;
+  auto fetch_stats = [&](uint32_t row) {
+    if (row >= r1) return;
+    if (next) st_ahead = __ldg(reinterpret_cast<const float2*>(a.stats) + row);
+    if constexpr (POST) ps_ahead = __ldg(reinterpret_cast<const float2*>(a.post_stats) + row);
+  };
+  fetch_stats(r0);
   for (uint32_t row = r0; row < r1; ++row) {
     if (!RING) fetch();
     if (row >= group_end) {  // a new group (or the first row)
@@ -195,8 +220,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       dx = static_cast<TS*>(g.dx.ptr) + b * g.dx.stride_b + t * g.dx.stride_t + col.first;
       if constexpr (JOIN) dy = static_cast<TB*>(g.dy.ptr) + b * g.dy.stride_b + t * g.dy.stride_t + col.first;
     }
-    if constexpr (RING) copy_async_wait();
+    if constexpr (RING) asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
     const float2 st = st_ahead, ps = ps_ahead;
+    fetch_stats(row + 1);
     // d: gradient of z, yh: yhat.  Columns outside the row stay zero.
     float d[K][VEC], yh[JOIN ? K : 1][VEC], zh[K][VEC], v[K][VEC];
     const float mr = st.x * st.y, pmr = ps.x * ps.y;
@@ -224,8 +250,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         vfma(zh[k], zh[k], a.residual_scale, q);
       }
       if constexpr (POST) {
-        G0.get(32 * k, q);
-        vadd(zh[k], zh[k], q);
+        if (bias) {
+          G0.get(32 * k, q);
+          vadd(zh[k], zh[k], q);
+        }
       }
       A.get(32 * k, q);
       vfma(zh[k], zh[k], st.y, -mr);
@@ -235,7 +263,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
       sum_on(s, v[k]);
       sum_on(sz, v[k], zh[k]);
     }
-    if (RING && row + 1 < r1) fetch();
+    if constexpr (RING) {
+      fetch_group();
+      if constexpr (DEPTH == 2) take_at = row_bytes - take_at;
+    }
     if (next) {
       const float2 m = team.sum2(s.x + s.y, sz.x + sz.y);
       const float m0 = a.next.kind == LVSA_BLOCK_NORM_LAYER ? st.y * (m.x * inv) : 0.f, m1 = st.y * (m.y * inv);
@@ -269,7 +300,8 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
         float q[VEC];
         G1.get(32 * k, q);
         vfma(P2[k], d[k], yh[k], P2[k]);
-        if constexpr (POST) vadd(Q2[k], Q2[k], d[k]);
+        if constexpr (POST)
+          if (bias) vadd(Q2[k], Q2[k], d[k]);
         vmul(d[k], d[k], q);
         if constexpr (POST) {
           sum_on(s, d[k]);
@@ -405,7 +437,7 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   static std::atomic<uint64_t> done{0}, last{0};
   const int64_t rows = static_cast<int64_t>(g.f.batch) * g.f.seq;
   const int shared = (FORM + 1) * shared_pitch(g.f.width) * static_cast<int>(sizeof(float)) +
-                     (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
+                     (VEC > 1 ? kDepth<FORM, VEC * K> * threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
   int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
   // A CTA ends with a piece of sums the size of some rows: not fewer than 8 rows each, unless SMs are left over.
