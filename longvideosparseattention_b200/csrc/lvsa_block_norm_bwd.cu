@@ -60,7 +60,7 @@ __device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t 
 
 // Rows on their way into shared memory.
 template <int FORM, int COLUMNS>
-constexpr int kDepth = FORM == 2 || COLUMNS > 8 ? 1 : 2;
+constexpr int kDepth = FORM == 2 || (FORM == 1 && COLUMNS > 8) ? 1 : 2;
 
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
 template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS, int CTAS>
@@ -474,6 +474,8 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
       !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC)) {
     return width <= 8 * 384 ? launch<TS, TB, FORM, 1, 8, 384, 1>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
   }
+  if constexpr (FORM == 0)
+    if (width <= 2048) return launch<TS, TB, FORM, VEC, 16 / VEC, 128, 4>(g, v, ctas, s);
   if (width <= 8 * 192) return launch<TS, TB, FORM, VEC, 8 / VEC, 192, FORM ? 3 : 4>(g, v, ctas, s);
   if (width <= 8 * 256) return launch<TS, TB, FORM, VEC, 8 / VEC, 256, FORM ? 2 : 3>(g, v, ctas, s);
   if (width <= 8 * 640) return launch<TS, TB, FORM, VEC, 8 / VEC, 640, 1>(g, v, ctas, s);
