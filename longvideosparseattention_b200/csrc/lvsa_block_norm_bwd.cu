@@ -369,47 +369,46 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
 // between CTAs k - 1 and k cuts; a group that no boundary cuts is done.  A
 // block takes 32 columns; its rows of threads share the CTAs and are added in
 // order.
-constexpr int kJoinRows = 32;
+constexpr int kJoinRows = 32;  // at most
 __global__ void __launch_bounds__(32 * kJoinRows) block_norm_sums_kernel(const __grid_constant__ BwdParams p) {
   const LvsaBlockNorm& a = p.g.f;
-  const int c = blockIdx.x * 32 + threadIdx.x;
-  int64_t first = 0, last = p.ctas, group = -1, start = 0;  // CTAs whose sums are added
+  const int c = blockIdx.x * 32 + threadIdx.x, width = a.width;
+  int first = 0, last = p.ctas, group = -1;  // CTAs whose sums are added
   int wanted = p.total_sums;
+  bool later = false;  // the group is not the first CTA's first
   if (blockIdx.y > 0) {
     wanted = p.piece_sums;
     const int64_t cut = p.groups <= static_cast<uint32_t>(p.ctas) ? 0 : first_row(p.rows, blockIdx.y, p.ctas);
     group = cut ? p.by_group.div(static_cast<uint32_t>(cut)) : blockIdx.y - 1;
-    start = group * p.by_group.d;
-    first = row_owner(p.rows, start, p.ctas);
-    last = row_owner(p.rows, start + p.by_group.d - 1, p.ctas) + 1;
+    const int64_t start = static_cast<int64_t>(group) * p.by_group.d;
+    first = static_cast<int>(row_owner(p.rows, start, p.ctas));
+    last = static_cast<int>(row_owner(p.rows, start + p.by_group.d - 1, p.ctas)) + 1;
     // Whole groups are done; of several cuts the first one's block is here.
-    if (last - first == 1 || (cut && (cut == start || blockIdx.y != first + 1))) return;
+    if (last - first == 1 || (cut && (cut == start || static_cast<int>(blockIdx.y) != first + 1))) return;
+    later = first_row(p.rows, first, p.ctas) < start;
   }
   if (!wanted) return;
   float sum[kSums] = {0.f, 0.f, 0.f, 0.f};
-  if (c < a.width) {
+  if (c < width) {
 #pragma unroll 4
-    for (int64_t i = first + threadIdx.y; i < last; i += kJoinRows) {
-      const float* from = p.totals + i * kSums * a.width;
-      if (group >= 0) {
-        const bool later = first_row(p.rows, i, p.ctas) < start;  // the group is not its CTA's first
-        from = p.pieces + (2 * i + later) * kSums * a.width;
-      }
+    for (int i = first + threadIdx.y; i < last; i += blockDim.y) {
+      const float* from = group < 0 ? p.totals + static_cast<int64_t>(i) * kSums * width
+                                    : p.pieces + (2 * static_cast<int64_t>(i) + (later && i == first)) * kSums * width;
 #pragma unroll
       for (int j = 0; j < kSums; ++j)
-        if (wanted >> j & 1) sum[j] += from[j * a.width + c];
+        if (wanted >> j & 1) sum[j] += from[j * width + c];
     }
   }
   __shared__ float part[kSums][kJoinRows][32];
 #pragma unroll
   for (int j = 0; j < kSums; ++j) part[j][threadIdx.y][threadIdx.x] = sum[j];
   __syncthreads();
-  if (threadIdx.y != 0 || c >= a.width) return;
+  if (threadIdx.y != 0 || c >= width) return;
 #pragma unroll
   for (int j = 0; j < kSums; ++j)
-    for (int i = 1; i < kJoinRows; ++i) sum[j] += part[j][i][threadIdx.x];
+    for (int i = 1; i < static_cast<int>(blockDim.y); ++i) sum[j] += part[j][i][threadIdx.x];
   if (group >= 0) {
-    const int64_t b = group / a.frames;
+    const int b = group / a.frames;
     store_group(p.g, b, group - b * a.frames, c, sum);
     return;
   }
@@ -455,7 +454,11 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   if (cudaGetLastError() != cudaSuccess) return LVSA_ERR_CUDA;
   if (!p.piece_sums && !p.total_sums) return LVSA_OK;
   const dim3 grid((g.f.width + 31) / 32, static_cast<unsigned>(groups <= ctas ? groups + 1 : ctas));
-  block_norm_sums_kernel<<<grid, dim3(32, kJoinRows), 0, s>>>(p);
+  // As many rows of threads as there are CTAs to add, a quarter of them each.
+  const int64_t added = p.total_sums ? ctas : ctas / groups + 2;
+  int join_rows = 4;
+  while (join_rows < kJoinRows && 4 * join_rows < added) join_rows *= 2;
+  block_norm_sums_kernel<<<grid, dim3(32, join_rows), 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
