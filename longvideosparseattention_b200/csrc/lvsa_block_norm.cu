@@ -42,7 +42,7 @@ struct FwdParams {
 };
 
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
-template <typename TS, typename TB, int FORM, int VEC, int K>
+template <typename TS, typename TB, int FORM, int VEC, int K, bool WHOLE>
 __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(const __grid_constant__ FwdParams p) {
   __shared__ float2 slots[2 * kMaxWarps];
   extern __shared__ float4 shared_vectors[];
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
   const int slot = (threadIdx.x >> 5) * K * 32 + (threadIdx.x & 31);
   RX* const x_slot = reinterpret_cast<RX*>(held + p.vectors_held * pitch) + slot;
   RY* const y_slot = reinterpret_cast<RY*>(x_slot - slot + K * blockDim.x) + slot;
-  Team team(slots, p.warps);
+  Team<WHOLE> team(slots, p.warps);
   const Columns<VEC, K> col(team, p.width);
   __shared__ float counts[kMaxWarps];
   const Held share(counts, col, team);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
 #pragma unroll
           for (int k = 0; k < K; ++k)
             if (col.in(k)) take_y(k, all[k]);
-          st = row_stats<VEC, K>(all, col, p.post_kind, p.post_eps, share, team);
+          st = row_stats(all, col, p.post_kind, p.post_eps, share, team);
           if (p.post_stats && team.warp == 0 && team.lane == 0) p.post_stats[row] = st;
         }
 #pragma unroll
@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
         h += teams * p.h.stride_t;
       }
       if (next) {
-        const float2 st = row_stats<VEC, K>(z, col, p.kind, p.eps, share, team);
+        const float2 st = row_stats(z, col, p.kind, p.eps, share, team);
         if (p.stats && team.warp == 0 && team.lane == 0) p.stats[row] = st;
         const float mr = st.x * st.y;
 #pragma unroll
@@ -223,9 +223,9 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
   const int vectors_held = !JOIN ? 2 : a.post.bias ? 4 : 3;
   const int shared = vectors_held * shared_pitch(a.width) * static_cast<int>(sizeof(float)) +
                      (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + (JOIN ? sizeof(TB) : 0)) : 0);
-  auto kern = block_norm_fwd_kernel<TS, TB, FORM, VEC, K>;
-  static std::atomic<uint64_t> done{0}, last{0};
-  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done, last);
+  auto kern = teams == 1 ? block_norm_fwd_kernel<TS, TB, FORM, VEC, K, true> : block_norm_fwd_kernel<TS, TB, FORM, VEC, K, false>;
+  static std::atomic<uint64_t> done[2], last[2];
+  const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done[teams == 1], last[teams == 1]);
   if (ctas < 1) return LVSA_ERR_CUDA;
   const FwdParams p{a.x, a.y, a.h, a.n, v, FastDiv(a.seq), FastDiv(a.seq / a.frames), static_cast<uint32_t>(rows),
                     static_cast<uint32_t>(a.frames), a.width, warps, vectors_held, a.next.kind, a.post.kind, a.residual_scale,

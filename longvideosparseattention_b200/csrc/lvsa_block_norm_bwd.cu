@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
   __shared__ float2 slots[2 * kMaxWarps];
   extern __shared__ float4 dynamic[];
   float* const held = reinterpret_cast<float*>(dynamic);
-  Team team(slots, blockDim.x >> 5);
+  Team<true> team(slots, blockDim.x >> 5);
   const LvsaBlockNormGrad& g = p.g;
   const LvsaBlockNorm& a = g.f;
   const Columns<VEC, K> col(team, a.width);

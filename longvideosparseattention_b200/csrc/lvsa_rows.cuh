@@ -257,7 +257,9 @@ constexpr int kMaxWarps = 32;  // of a CTA
 // their own in shared memory, a hardware barrier of their own.  One barrier a
 // sum: the slots alternate, and a thread that writes a slot again has passed
 // the barrier of the sum between, which every reader of the slot has reached
-// after reading it.
+// after reading it.  WHOLE: the team is its CTA (a barrier whose number is only
+// known at run time costs a CTA all sixteen, and an SM has room for four such).
+template <bool WHOLE>
 struct Team {
   float* slots;
   int count, round, warp, lane, barrier, turn;  // round: the power of two at or above count
@@ -277,7 +279,7 @@ struct Team {
     return s;
   }
   __device__ __forceinline__ void sync() {
-    if (count * 32 == blockDim.x) __syncthreads();
+    if constexpr (WHOLE) __syncthreads();
     else asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(count * 32) : "memory");
   }
   // Over the team, of what lane l holds of warp l modulo `round`.
@@ -310,7 +312,8 @@ template <int VEC, int K>
 struct Columns {
   static constexpr int kStep = 32 * VEC;
   int first, width;
-  __device__ __forceinline__ Columns(const Team& t, int w) : first((t.warp * K * 32 + t.lane) * VEC), width(w) {}
+  template <bool WHOLE>
+  __device__ __forceinline__ Columns(const Team<WHOLE>& t, int w) : first((t.warp * K * 32 + t.lane) * VEC), width(w) {}
   __device__ __forceinline__ int at(int k) const { return first + k * kStep; }
   __device__ __forceinline__ bool in(int k) const { return first + k * kStep < width; }
   // Values of the row that warp w holds.
@@ -372,8 +375,8 @@ __device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_
 struct Held {
   const float* counts;
   float inv_mine, inv_row;
-  template <int VEC, int K>
-  __device__ __forceinline__ Held(float* space, const Columns<VEC, K>& col, const Team& team) : counts(space) {
+  template <int VEC, int K, bool WHOLE>
+  __device__ __forceinline__ Held(float* space, const Columns<VEC, K>& col, const Team<WHOLE>& team) : counts(space) {
     if (team.lane < team.count) space[team.lane] = col.of_warp(team.lane);
     __syncthreads();
     inv_mine = 1.f / fmaxf(space[team.warp], 1.f);
@@ -384,9 +387,9 @@ struct Held {
 // Mean (0 for the RMS norm) and 1 / sqrt(variance + eps) of a row.  The layer
 // norm's sums are joined from each warp's own mean and squares about it, so
 // that a row's offset does not cancel in the variance, with one barrier.
-template <int VEC, int K>
+template <int VEC, int K, bool WHOLE>
 __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Columns<VEC, K>& col, int kind, float eps,
-                                            const Held& held, Team& team) {
+                                            const Held& held, Team<WHOLE>& team) {
   float2 run = make_float2(0.f, 0.f);
   if (kind == LVSA_BLOCK_NORM_RMS) {
 #pragma unroll
