@@ -52,6 +52,8 @@ struct W4Params {
   int32_t chunk;          // k tiles of each stretch for which x is held at once
   int32_t pitch;          // 16 bytes between the columns of x held
   int32_t x_vectors;      // x may be read 8 values at a time
+  FastDiv by_octets;      // by the groups of 8 values of a row of x that are held
+  FastDiv by_slots;       // by the outputs of a row of x of a turn
 };
 
 // ---- layout: lane l = 4 r + j of a tile holds rows r and r + 8, columns
@@ -104,14 +106,20 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
 
   // x's columns of chunk `first` of every stretch, as digits, and their powers
   // of two: a thread takes 8 values, the threads of a block agree on a power.
+  const bool whole = p.chunk >= p.stretch;  // all of x is held
+  const int octets = p.splits * p.chunk * (kTileK / 8);
   auto stage = [&](int first) {
-    const int held = p.splits * p.chunk, octets = held * (kTileK / 8);
     constexpr int kLanes = HALVES ? 4 : 8;  // threads a block
     for (int i = threadIdx.x; i < (rows * octets + 31) / 32 * 32; i += kThreads) {
-      const int m = i / octets, o = i - m * octets;  // octets is a multiple of 8: a block lies in one row
-      const int at = o / 8, stretch = at / p.chunk, tile = first + at - stretch * p.chunk;
-      const int64_t k0 = static_cast<int64_t>(stretch * p.stretch + tile) * kTileK + o % 8 * 8;
-      const int64_t end = tile < p.stretch && m < rows ? a.k : 0;  // past a stretch's end: zeros, not used
+      const int m = p.by_octets.div(i), o = i - m * octets, at = o / 8;  // octets is a multiple of 8: a block lies in one row
+      int tile = at, end = m < rows ? a.k : 0;
+      if (!whole) {
+        const int stretch = at / p.chunk;
+        tile = first + at - stretch * p.chunk;
+        if (tile >= p.stretch) end = 0;  // past a stretch's end: zeros, not used
+        tile += stretch * p.stretch;
+      }
+      const int k0 = tile * kTileK + o % 8 * 8;
       float v[8];
       if (p.x_vectors && k0 + 8 <= end) {
         any_load<8>(a.x, a.x_dtype, (m0 + m) * a.ldx + k0, v);
@@ -135,18 +143,18 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       float up = most < 0x7f800000u ? __uint_as_float((power - 25u) << 23) : __uint_as_float(0x7fc00000u);
       // Rounded to a whole number by 1.5 2^23, and with 128 (1 + 256 + 65536)
       // more, the bytes of it are the digits + 128.
-      uint32_t whole[8];
+      uint32_t number[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        whole[e] = (__float_as_uint(fmaf(v[e], down, kMagicValue)) - (kMagic - 0x00808080u)) ^ 0x00808080u;
+        number[e] = (__float_as_uint(fmaf(v[e], down, kMagicValue)) - (kMagic - 0x00808080u)) ^ 0x00808080u;
 #pragma unroll
       for (int digit = 0; digit < kDigits; ++digit) {
         uint32_t packed[2];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {  // byte `digit` of four numbers
           const uint32_t pick = digit | (digit + 4) << 4;
-          packed[q] = __byte_perm(__byte_perm(whole[4 * q], whole[4 * q + 1], pick),
-                                  __byte_perm(whole[4 * q + 2], whole[4 * q + 3], pick), 0x5410);
+          packed[q] = __byte_perm(__byte_perm(number[4 * q], number[4 * q + 1], pick),
+                                  __byte_perm(number[4 * q + 2], number[4 * q + 3], pick), 0x5410);
         }
         const int c = m * kDigits + digit;
         if (m < rows) {  // lane j's 16 bytes: its 8 columns of either half of the tile
@@ -170,7 +178,6 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
   const int column_tiles = (cols + 7) / 8;
   const int scale_lane = split * p.chunk * kBlocks * kCols + 2 * j;
 
-  const bool whole = p.chunk >= p.stretch;
   const int turns = (p.row_tiles + gridDim.x * p.slots - 1) / (gridDim.x * p.slots);
   for (int turn = 0; turn < turns; ++turn) {
     // Neighbouring CTAs take neighbouring rows of tiles: the SMs' shares differ by one at most.
@@ -286,7 +293,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       }
     __syncthreads();
     for (int i = threadIdx.x; i < p.slots * rows * kTileN; i += kThreads) {
-      const int row = i % kTileN, m = i / kTileN % rows, which = i / (kTileN * rows);
+      const int m = p.by_slots.div(i), row = i % kTileN, which = (i - m * p.slots * kTileN) / kTileN;
       const int64_t n = static_cast<int64_t>((turn * p.slots + which) * gridDim.x + blockIdx.x) * kTileN + row;
       if (n >= a.n) continue;
       float sum = 0.f;
@@ -335,6 +342,8 @@ int launch(W4Params p, cudaStream_t s) {
     if (p.splits == 1) return LVSA_ERR_UNSUPPORTED;
   }
   p.pitch = column_pitch(p.splits * p.chunk);
+  p.by_octets = FastDiv(p.splits * p.chunk * (kTileK / 8));
+  p.by_slots = FastDiv(p.slots * kTileN);
   auto kern = w4_linear_kernel<NT, HALVES, TSc>;
   const int shared = shared_of();
   static std::atomic<uint64_t> done{0};
