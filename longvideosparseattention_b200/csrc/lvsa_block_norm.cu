@@ -243,7 +243,7 @@ int launch_width(const LvsaBlockNorm& a, cudaStream_t s) {
       rows_vector<TB, VEC>(a.n) && v.aligned(VEC)) {
     // The fewest warps of kElems values a thread, then the fewest values; half
     // of kElems where the rows do not fill the device and a row's latency is
-    // the time (2 x 77 rows of 2048: 4.5 us with 32 values, FEW_US with 16).
+    // the time (2 x 77 rows of 2048: 4.5 us with 32 values, 4.2 with 16).
     const int vectors = a.width / VEC, warps = (vectors * VEC + 32 * kElems - 1) / (32 * kElems);
     constexpr int kMost = kElems / VEC;
     const bool few = static_cast<int64_t>(a.batch) * a.seq <= 4 * device_sms();

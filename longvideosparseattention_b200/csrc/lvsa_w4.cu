@@ -40,7 +40,7 @@ constexpr int kMaxShared = 227 * 1024 - 1024;
 // 19.7, 6 19.9; 32 with 4 19.8, with 3 20.3; prefetching further to L2 is slower
 // (8 tiles more 20.6, 16 22.0).
 template <int NT>
-constexpr int kWarpsW4 = NT <= 4 ? 28 : 20;
+constexpr int kWarpsW4 = NT <= 2 ? 28 : 16;
 constexpr int kAhead = 4;
 
 struct W4Params {
@@ -235,27 +235,36 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
           f[h >> 1][2 * (h & 1)] = words[h] & kHigh;
           f[h >> 1][2 * (h & 1) + 1] = words[h] << 4 & kHigh;
         }
+        // Two tiles of columns side by side, so that one's products run while
+        // the other's sums wait; a last odd one has a neighbour not used.
+        constexpr int kSide = NT > 1 ? 2 : 1;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          if (NT > 2 && t >= column_tiles) break;
-          const uint4 b = shared_w4[x_at[t] + u * 4];
+        for (int t0 = 0; t0 < NT; t0 += kSide) {
+          if (NT > kSide && t0 >= column_tiles) break;
           const int magic[4] = {kMagic, kMagic, kMagic, kMagic};
-          int sum[4];
+          int sum[kSide][4];
+          uint4 b[kSide];
           auto add = [&](int block) {
-            const float2 up = *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc[t][i] += (i < 2 ? lo : hi)[block] * ((__int_as_float(sum[i]) - kMagicValue) * (i & 1 ? up.y : up.x));
+            for (int q = 0; q < kSide; ++q) {
+              const float2 up =
+                  *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * (t0 + q));
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[t0 + q][i] += (i < 2 ? lo : hi)[block] * ((__int_as_float(sum[q][i]) - kMagicValue) * (i & 1 ? up.y : up.x));
+            }
           };
-          mma(sum, f[0], b.x, b.y, magic);
-          if constexpr (HALVES) {
-            add(0);
-            mma(sum, f[1], b.z, b.w, magic);
-            add(1);
-          } else {
-            mma(sum, f[1], b.z, b.w, sum);
-            add(0);
+#pragma unroll
+          for (int q = 0; q < kSide; ++q) b[q] = shared_w4[x_at[t0 + q] + u * 4];
+#pragma unroll
+          for (int q = 0; q < kSide; ++q) mma(sum[q], f[0], b[q].x, b[q].y, magic);
+          if constexpr (HALVES) add(0);
+#pragma unroll
+          for (int q = 0; q < kSide; ++q) {
+            if constexpr (HALVES) mma(sum[q], f[1], b[q].z, b[q].w, magic);
+            else mma(sum[q], f[1], b[q].z, b[q].w, sum[q]);
           }
+          add(kBlocks - 1);
         }
         if (more) {
           w[u] = __ldg(tiles + (u + kAhead) * 32);
