@@ -12,8 +12,8 @@ The Wan, HunyuanVideo and CogVideoX blocks run ``norm_modulate`` before
 attention and MLP and ``gate_residual`` after each; with sandwich norms the
 branch is normalised first (``post_norm``).
 
-Tensors: ``x`` (the residual stream) and ``h`` [B, S, C] in bf16, fp16 or
-fp32; ``y`` (the branch) and ``n`` of the same type, or bf16 / fp16 beside an
+Tensors: ``x`` (the residual stream) and ``h`` [B, S, C], C up to 8192, in bf16,
+fp16 or fp32; ``y`` (the branch) and ``n`` of the same type, or bf16 / fp16 beside an
 fp32 stream.  ``scale``, ``shift`` and ``gate`` are [C], [B, C] or [B, F, C]
 (B or F may be 1) in any of the three types: with F frames, token s takes the
 vector of frame s // (S / F).  Norms: ``"layer"`` (weight and bias optional) or
@@ -21,7 +21,9 @@ vector of frame s // (S / F).  Norms: ``"layer"`` (weight and bias optional) or
 rounding of each output; ``n`` is of ``h`` before its rounding.
 
 All three are differentiable in every tensor (once); gradients of vectors are
-fp32 sums in a fixed order, so a step repeats bit for bit.
+fp32 sums in a fixed order, so a step repeats bit for bit.  Calls run on the
+current stream and can be captured into a CUDA graph, a backward pass with
+them (``torch.autograd.grad``, after a first step outside the capture).
 """
 
 from __future__ import annotations

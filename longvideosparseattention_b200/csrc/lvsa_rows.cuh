@@ -438,6 +438,10 @@ __device__ __forceinline__ float2 row_stats(const float (&z)[K][VEC], const Colu
   return make_float2(mean, rsqrtf(q * held.inv_row + eps));
 }
 
+// Sums over rows that the backward keeps for each CTA in its workspace: three
+// times (two pieces, and the totals) as many vectors of the channels.
+constexpr int kBlockNormSums = 4;
+
 // Rows [first_row(i), first_row(i + 1)) are CTA i's of n; row_owner is its inverse.
 __host__ __device__ __forceinline__ int64_t first_row(int64_t rows, int64_t i, int64_t n) { return rows * i / n; }
 __host__ __device__ __forceinline__ int64_t row_owner(int64_t rows, int64_t row, int64_t n) {

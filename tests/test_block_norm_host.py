@@ -65,7 +65,7 @@ def test_forward_checks():
         assert _fwd(_args(**bad)) == N.LVSA_ERR_INVALID_ARG, bad
     assert _fwd(_args(seq=7, frames=2)) == N.LVSA_ERR_GEOMETRY
     for bad in (dict(width=N.LVSA_BLOCK_NORM_MAX_WIDTH + 1), dict(stream_dtype=9), dict(branch_dtype=N.LVSA_DTYPE_E4M3),
-                dict(stream_dtype=N.LVSA_DTYPE_BF16, branch_dtype=N.LVSA_DTYPE_F32),
+                dict(batch=2, seq=2 ** 30), dict(stream_dtype=N.LVSA_DTYPE_BF16, branch_dtype=N.LVSA_DTYPE_F32),
                 dict(gate=N.LvsaVectors(FAKE, 0, 0, N.LVSA_DTYPE_E4M3, 0))):
         assert _fwd(_args(**bad)) == N.LVSA_ERR_UNSUPPORTED, bad
     norm = N.LvsaRowNorm

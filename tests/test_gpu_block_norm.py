@@ -377,6 +377,64 @@ def test_other_stream_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_second_derivative_is_refused():
+    """create_graph gives first derivatives; differentiating those raises rather than giving zeros."""
+    from longvideosparseattention_b200.block_norm import gate_residual_norm
+    g = torch.Generator().manual_seed(3)
+    x, y = _make((1, 4, 64), F32, g).requires_grad_(True), _make((1, 4, 64), F32, g)
+    h, n = gate_residual_norm(x, y)
+    first, = torch.autograd.grad(h.sum() + (n * n).sum(), x, create_graph=True)
+    h, n = gate_residual_norm(x, y)
+    again, = torch.autograd.grad(h.sum() + (n * n).sum(), x)
+    assert torch.equal(first.detach(), again)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.sum(), x)
+
+
+def test_saved_tensors():
+    """Saved tensors that a hook keeps elsewhere and brings back to other places; and one changed in place."""
+    t = _inputs(1, 30, 3, 264, BF, BF, F32, "layer", True, "rms", 5, True)
+    leaves = {k: v.requires_grad_(True) for k, v in t.items()}
+    h, n = _call(leaves, "layer", "rms", 1.0, BF)
+    want = torch.autograd.grad([h, n], list(leaves.values()), [h.detach(), n.detach()])
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: v.cpu(), lambda v: v.cuda()):
+        h, n = _call(leaves, "layer", "rms", 1.0, BF)
+    got = torch.autograd.grad([h, n], list(leaves.values()), [h.detach(), n.detach()])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    h, n = _call(leaves, "layer", "rms", 1.0, BF)
+    with torch.no_grad():
+        t["scale"].add_(1)
+    with pytest.raises(RuntimeError):
+        n.sum().backward()
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values: the last rows, forward and backward."""
+    from longvideosparseattention_b200.block_norm import gate_residual_norm
+    C, S = 8192, 2 ** 18 + 5
+    g = torch.Generator().manual_seed(12)
+    x, y = (torch.zeros(1, S, C, dtype=BF, device="cuda") for _ in range(2))
+    last = 3
+    x[:, -last:], y[:, -last:] = _make((1, last, C), BF, g), _make((1, last, C), BF, g)
+    gate, shift = _make((C,), F32, g), _make((C,), F32, g)
+    short = [v[:, -last:].clone() for v in (x, y)]
+    for v in (x, y, gate):
+        v.requires_grad_(True)
+    h, n = gate_residual_norm(x, y, gate, shift=shift)
+    dn = torch.zeros_like(n)
+    dn[:, -last:] = _make((1, last, C), BF, g)
+    dx, dy, dgate = torch.autograd.grad(n, (x, y, gate), dn)
+    assert torch.equal(n[0, 0], shift.bfloat16()) and torch.equal(n[0, 2 ** 17], shift.bfloat16())
+    sx, sy, sg = short[0].requires_grad_(True), short[1].requires_grad_(True), gate.detach().requires_grad_(True)
+    sh, sn = gate_residual_norm(sx, sy, sg, shift=shift)
+    ex, ey, eg = torch.autograd.grad(sn, (sx, sy, sg), dn[:, -last:])
+    # The same rows by the same kernels, in another order of the sums of a row: a step of bf16, and fp32's.
+    for a, b in ((h[:, -last:], sh), (n[:, -last:], sn), (dx[:, -last:], ex), (dy[:, -last:], ey)):
+        assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4).all()
+    assert ((dgate - eg).abs() <= 1e-4 * (1 + eg.abs())).all()
+    assert not dx[:, : -last].any() and not dy[:, : -last].any()
+
+
 def test_refusals_on_cuda_tensors():
     from longvideosparseattention_b200.block_norm import gate_residual, gate_residual_norm, norm_modulate
     x = torch.zeros(2, 6, 16, device="cuda")

@@ -133,6 +133,20 @@ def test_quantize():
         assert (back[3] == 0).all()
 
 
+def test_offsets_past_32_bits():
+    """Weights of more than 2^31 bytes of tiles: the first and the last outputs."""
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    n, k, group = 2 ** 18 + 20, 16448, 128
+    g = torch.Generator(device="cuda").manual_seed(1)
+    codes = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8, device="cuda")
+    scales = (torch.rand(n, -(-k // group), generator=g, device="cuda") / 128).bfloat16()
+    x = torch.randn(2, k, generator=g, device="cuda")
+    y = linear_w4(x, pack_w4(codes, scales, group))
+    for part in (slice(0, 40), slice(n - 40, n)):
+        want, size = _want(x, codes[part], scales[part], group, None, None)
+        _check(y[:, part], want, size)
+
+
 def test_infinities_and_large_rows():
     from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
     codes, scales = _make(64, 256, 64, BF, 5)
