@@ -75,7 +75,7 @@ def gate_residual_norm(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Te
 # ------------------------------------------------------------------ arguments
 class _Form:
     """What a call does, apart from its tensors."""
-    __slots__ = ("where", "join", "next", "post_kind", "post_eps", "kind", "eps", "alpha", "branch", "frames")
+    __slots__ = ("join", "next", "post_kind", "post_eps", "kind", "eps", "alpha", "branch", "frames")
 
 
 _ABSENT = (0, 0, 0, 0, 0)
@@ -112,13 +112,6 @@ def _channel(where: str, name: str, t: torch.Tensor, C: int, device: int) -> tor
     return t if C == 1 or t.stride(0) == 1 else t.contiguous()
 
 
-def _kind(where: str, name: str, kind: Optional[str]) -> int:
-    code = _KINDS.get(kind)
-    if code is None:
-        raise ValueError(f"{where}: {name} must be 'layer' or 'rms', got {kind!r}")
-    return code
-
-
 def _run(where, x, y, gate, alpha, post_norm, post_weight, post_bias, post_eps, norm, weight, bias, scale, shift, eps,
          out_dtype):
     if not x.is_cuda:
@@ -130,16 +123,16 @@ def _run(where, x, y, gate, alpha, post_norm, post_weight, post_bias, post_eps, 
         raise ValueError(f"{where}: x must be [B, S, C] with C of 1 to {N.LVSA_BLOCK_NORM_MAX_WIDTH}, got {tuple(shape)}")
     B, S, C = shape
     form = _Form()
-    form.where, form.join, form.next = where, y is not None, where != "gate_residual"
+    form.join, form.next = y is not None, where != "gate_residual"
     form.alpha, form.eps, form.post_eps = float(alpha), float(eps), float(post_eps)
     if not (form.eps >= 0 and form.post_eps >= 0):
         raise ValueError(f"{where}: eps must not be negative")
-    form.kind = _kind(where, "norm", norm) if form.next else 0
-    form.post_kind = _kind(where, "post_norm", post_norm) if post_norm is not None else 0
-    if (bias is not None and norm != "layer") or (post_bias is not None and post_norm != "layer"):
-        raise ValueError(f"{where}: only a layer norm has a bias")
-    if post_weight is not None and not form.post_kind:
-        raise ValueError(f"{where}: post_weight without post_norm")
+    form.kind = _KINDS.get(norm, 0)
+    form.post_kind = _KINDS.get(post_norm, 0)
+    if form.next and not form.kind:
+        raise ValueError(f"{where}: norm must be 'layer' or 'rms', got {norm!r}")
+    if post_norm is not None and not form.post_kind:
+        raise ValueError(f"{where}: post_norm must be None, 'layer' or 'rms', got {post_norm!r}")
     if form.join:
         _typed(where, "y", y, device)
         if y.shape != shape:
@@ -170,10 +163,16 @@ def _run(where, x, y, gate, alpha, post_norm, post_weight, post_bias, post_eps, 
     if weight is not None:
         weight = _channel(where, "weight", weight, C, device)
     if bias is not None:
+        if norm != "layer":
+            raise ValueError(f"{where}: only a layer norm has a bias")
         bias = _channel(where, "bias", bias, C, device)
     if post_weight is not None:
+        if not form.post_kind:
+            raise ValueError(f"{where}: post_weight without post_norm")
         post_weight = _channel(where, "post_weight", post_weight, C, device)
     if post_bias is not None:
+        if post_norm != "layer":
+            raise ValueError(f"{where}: only a layer norm has a bias")
         post_bias = _channel(where, "post_bias", post_bias, C, device)
     tensors = (x, y, gate, scale, shift, weight, bias, post_weight, post_bias)
     if torch.is_grad_enabled():
@@ -208,29 +207,34 @@ def _full(v: Optional[torch.Tensor], full: Tuple[int, int, int]) -> Optional[tor
 def _row_args(t: Optional[torch.Tensor]) -> Tuple[int, int, int]:
     if t is None:
         return _NO_ROWS
-    shape, stride = t.shape, t.stride()
-    return t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0
+    B, S, _ = t.shape
+    stride_b, stride_t, _ = t.stride()
+    return t.data_ptr(), stride_b if B > 1 else 0, stride_t if S > 1 else 0
 
 
 def _vector_args(t: Optional[torch.Tensor]) -> Tuple[int, int, int, int, int]:
     if t is None:
         return _ABSENT
+    n = t.dim()
+    if n == 1:
+        return t.data_ptr(), 0, 0, _DT[t.dtype], 0
     shape, stride = t.shape, t.stride()
-    n = len(shape)
-    return (t.data_ptr(), stride[0] if n > 1 and shape[0] > 1 else 0, stride[1] if n == 3 and shape[1] > 1 else 0,
+    return (t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if n == 3 and shape[1] > 1 else 0,
             _DT[t.dtype], 0)
 
 
 def _norm_args(kind: int, eps: float, w: Optional[torch.Tensor], b: Optional[torch.Tensor]):
+    if w is None and b is None:
+        return kind, eps, 0, 0, 0, 0
     return (kind, eps, 0 if w is None else _DT[w.dtype], 0 if b is None else _DT[b.dtype],
             0 if w is None else w.data_ptr(), 0 if b is None else b.data_ptr())
 
 
-def _args(form: _Form, tensors, h, n, stats, post_stats) -> tuple:
-    """LvsaBlockNorm's fields."""
+def _args(form: _Form, tensors, h: int, n: int, stats, post_stats) -> tuple:
+    """LvsaBlockNorm's fields; h, n: addresses of contiguous outputs."""
     x, y, gate, scale, shift, weight, bias, post_weight, post_bias = tensors
     B, S, C = x.shape
-    return (*_row_args(x), *_row_args(y), *_row_args(h), *_row_args(n), *_vector_args(gate), *_vector_args(scale),
+    return (*_row_args(x), *_row_args(y), h, S * C, C, n, S * C, C, *_vector_args(gate), *_vector_args(scale),
             *_vector_args(shift), *_norm_args(form.post_kind, form.post_eps, post_weight, post_bias),
             *_norm_args(form.kind, form.eps, weight, bias), form.alpha, _DT[x.dtype], _DT[form.branch], B, S,
             form.frames, C, 0 if stats is None else stats.data_ptr(), 0 if post_stats is None else post_stats.data_ptr())
@@ -239,14 +243,16 @@ def _args(form: _Form, tensors, h, n, stats, post_stats) -> tuple:
 def _forward(form: _Form, tensors, keep: bool):
     """(h or None, n or None, stats, post_stats); the statistics only where ``keep``."""
     x = tensors[0]
-    shape, device = x.shape, x.device
-    h = torch.empty(shape, dtype=x.dtype, device=device) if form.join else None
-    n = torch.empty(shape, dtype=form.branch, device=device) if form.next else None
+    shape = x.shape
+    h = x.new_empty(shape) if form.join else None
+    n = x.new_empty(shape, dtype=form.branch) if form.next else None
     rows = shape[0] * shape[1]
-    stats = torch.empty(rows, 2, dtype=torch.float32, device=device) if keep and form.next else None
-    post_stats = torch.empty(rows, 2, dtype=torch.float32, device=device) if keep and form.post_kind else None
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if keep and form.next else None
+    post_stats = x.new_empty((rows, 2), dtype=torch.float32) if keep and form.post_kind else None
     if rows:
-        launch("lvsa_block_norm_fwd", BLOCK_NORM.pack(*_args(form, tensors, h, n, stats, post_stats)), x.get_device())
+        launch("lvsa_block_norm_fwd", BLOCK_NORM.pack(*_args(
+            form, tensors, 0 if h is None else h.data_ptr(), 0 if n is None else n.data_ptr(), stats, post_stats)),
+            x.get_device())
     return h, n, stats, post_stats
 
 
@@ -288,10 +294,10 @@ def _backward(ctx, dh, dn):
         totals = [0 if t is None else t.data_ptr() for t in (dw, db, dpw, dpb)]
         device = x.get_device()
         size = _workspace(x.dtype, form.branch, B, S, form.frames, C, form.post_kind != 0, form.join, any(totals), device)
-        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+        space = x.new_empty((size,), dtype=torch.uint8)
         # n is set where there is a next norm, and not read.
         args = BLOCK_NORM_GRAD.pack(
-            *_args(form, tensors, None, x if form.next else None, stats, post_stats),
+            *_args(form, tensors, 0, x.data_ptr() if form.next else 0, stats, post_stats),
             *_row_args(None if dh is None else _rows(dh)), *_row_args(None if dn is None else _rows(dn)),
             *_row_args(dx), *_row_args(dy), *_vector_args(dgate), *_vector_args(dscale), *_vector_args(dshift), *totals,
             space.data_ptr(), size)
