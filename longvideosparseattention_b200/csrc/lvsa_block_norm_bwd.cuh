@@ -64,8 +64,8 @@ __device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t 
 }
 
 // Rows on their way into shared memory.
-template <int FORM, int COLUMNS>
-constexpr int kDepth = FORM == 2 || (FORM == 1 && COLUMNS > 8) ? 1 : 2;
+template <int FORM, int THREADS>
+constexpr int kDepth = FORM == 2 || (FORM == 1 && THREADS == 512) ? 1 : 2;
 
 // FORM 0: the norm alone; 1: a join; 2: a join with a norm of the branch.
 template <typename TS, typename TB, int FORM, int VEC, int K, int THREADS, int CTAS>
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
   typename PB::R* const ys = ns + K * blockDim.x;
   // Two rows on their way, in turn (77910 x 2048 with a join 370 us with one
   // row, 325 with two; with a norm of the branch 444 and 510 at 17550 x 5120).
-  constexpr int DEPTH = kDepth<FORM, VEC * K>;
+  constexpr int DEPTH = kDepth<FORM, THREADS>;
   const int row_bytes = K * blockDim.x * static_cast<int>(sizeof(xs[0]) + sizeof(ns[0])) * (JOIN ? 2 : 1);
   int put_at = 0, take_at = 0;  // bytes to the row to fetch, and to take
   auto slot_of = [&](auto* slot, int k, int at) {
@@ -443,7 +443,7 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   static std::atomic<uint64_t> done{0}, last{0};
   const int64_t rows = static_cast<int64_t>(g.f.batch) * g.f.seq;
   const int shared = (FORM + 1) * shared_pitch(g.f.width) * static_cast<int>(sizeof(float)) +
-                     (VEC > 1 ? kDepth<FORM, VEC * K> * threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
+                     (VEC > 1 ? kDepth<FORM, THREADS> * threads * K * VEC * static_cast<int>(sizeof(TS) + sizeof(TB)) * (FORM ? 2 : 1) : 0);
   int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done, last);
   if (ctas < 1) return LVSA_ERR_CUDA;
   // A CTA ends with a piece of sums the size of some rows: not fewer than 8 rows each, unless SMs are left over.
@@ -469,10 +469,12 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
-// 8 columns a thread up to 5120 channels, 16 beyond and for the norm alone up
-// to 2048, whose rows' own instructions weigh more (126360 x 1536: 287 us with
-// 8, 251 with 16); the fewer threads a CTA may have, the more registers they
-// get.  Value by value where the accesses of a vector do not fit.
+// 8 columns a thread up to 5120 channels, 16 beyond and where rows' own
+// instructions weigh more: the norm alone up to 2048 (126360 x 1536: 287 us with
+// 8, 251 with 16), a join of 1025 to 1536 (131040 x 1536: 437 and 414, with a norm
+// of the branch 633 and 554; 77910 x 2048: 314 and 326; 100000 x 512: 124 and
+// 131).  The fewer threads a CTA may have, the more registers they get.  Value
+// by value where the accesses of a vector do not fit.
 template <typename TS, typename TB, int FORM>
 int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   constexpr int VEC = kVec<TS>;
@@ -488,7 +490,8 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
   if constexpr (FORM == 0) {
     if (width <= 16 * 128) return launch<TS, TB, FORM, VEC, 16 / VEC, 128, 4>(g, v, ctas, s);
   } else {
-    if (width <= 8 * 192) return launch<TS, TB, FORM, VEC, 8 / VEC, 192, 3>(g, v, ctas, s);
+    if (width <= 8 * 128) return launch<TS, TB, FORM, VEC, 8 / VEC, 128, 4>(g, v, ctas, s);
+    if (width <= 16 * 96) return launch<TS, TB, FORM, VEC, 16 / VEC, 96, 4>(g, v, ctas, s);
     if (width <= 8 * 256) return launch<TS, TB, FORM, VEC, 8 / VEC, 256, 2>(g, v, ctas, s);
   }
   if (width <= 8 * 640) return launch<TS, TB, FORM, VEC, 8 / VEC, 640, 1>(g, v, ctas, s);
