@@ -46,20 +46,26 @@ struct BwdParams {
   float* totals;
 };
 
-// What a group's sums give at column c; b, f: the group's.
-__device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, int64_t b, int64_t f, int c, const float (&q)[kSums]) {
-  const LvsaBlockNorm& a = g.f;
-  const int64_t at = (b * a.frames + f) * a.width + c;
-  if (g.dshift.ptr) any_store(g.dshift.ptr, g.dshift.dtype, at, q[1]);
+// What a group's sums (P, Q, P2, Q2) give at VEC columns from c; b, f: the group's.
+template <int VEC>
+__device__ __forceinline__ void store_group(const LvsaBlockNormGrad& g, const Vectors& v, int64_t b, int64_t f, int c,
+                                            const float (&q)[kSums][VEC]) {
+  const int64_t at = (b * g.f.frames + f) * g.f.width + c;
+  float w[VEC], o[VEC];
+  if (g.dshift.ptr) any_store<VEC>(g.dshift.ptr, g.dshift.dtype, at, q[1]);
   if (g.dscale.ptr) {
-    const float w = a.next.weight ? any_load(a.next.weight, a.next.weight_dtype, c) : 1.f;
-    const float o = a.next.bias ? any_load(a.next.bias, a.next.bias_dtype, c) : 0.f;
-    any_store(g.dscale.ptr, g.dscale.dtype, at, w * q[0] + o * q[1]);
+    vector_or<VEC>(v.weight, 0, 0, c, 1.f, w);
+    vector_or<VEC>(v.bias, 0, 0, c, 0.f, o);
+    vmul(o, o, q[1]);
+    vfma(w, w, q[0], o);
+    any_store<VEC>(g.dscale.ptr, g.dscale.dtype, at, w);
   }
   if (g.dgate.ptr) {
-    const float w = a.post.weight ? any_load(a.post.weight, a.post.weight_dtype, c) : 1.f;
-    const float o = a.post.bias ? any_load(a.post.bias, a.post.bias_dtype, c) : 0.f;
-    any_store(g.dgate.ptr, g.dgate.dtype, at, w * q[2] + o * q[3]);
+    vector_or<VEC>(v.post_weight, 0, 0, c, 1.f, w);
+    vector_or<VEC>(v.post_bias, 0, 0, c, 0.f, o);
+    vmul(o, o, q[3]);
+    vfma(w, w, q[2], o);
+    any_store<VEC>(g.dgate.ptr, g.dgate.dtype, at, w);
   }
 }
 
@@ -343,28 +349,41 @@ __global__ void __launch_bounds__(THREADS, CTAS) block_norm_bwd_kernel(const __g
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!col.in(k)) continue;
+      const int c = col.at(k);
+      float q[kSums][VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const int c = col.at(k) + e;
-        float q[kSums] = {P[k][e], Q[k][e], 0.f, 0.f};
-        if constexpr (JOIN) q[2] = P2[k][e];
-        if constexpr (POST) q[3] = Q2[k][e];
-        if (whole) {
-          store_group(g, b, f, c, q);
-        } else {
+        q[0][e] = P[k][e];
+        q[1][e] = Q[k][e];
+        q[2][e] = q[3][e] = 0.f;
+        if constexpr (JOIN) q[2][e] = P2[k][e];
+        if constexpr (POST) q[3][e] = Q2[k][e];
+      }
+      if (whole) {
+        store_group<VEC>(g, p.v, b, f, c, q);
+      } else {
 #pragma unroll
-          for (int i = 0; i < kSums; ++i)
-            if (p.piece_sums >> i & 1) piece[i * a.width + c] = q[i];
-        }
-        if (p.total_sums) {
-          const int64_t fs = b * a.scale.stride_b + f * a.scale.stride_f + c, fg = b * a.gate.stride_b + f * a.gate.stride_f + c;
-          const float up = a.scale.ptr ? 1.f + any_load(a.scale.ptr, a.scale.dtype, fs) : 1.f;
-          const float gt = a.gate.ptr ? any_load(a.gate.ptr, a.gate.dtype, fg) : 1.f;
+        for (int i = 0; i < kSums; ++i)
+          if (p.piece_sums >> i & 1) any_store<VEC>(piece, LVSA_DTYPE_F32, i * a.width + c, q[i]);
+      }
+      if (p.total_sums) {
+        float up[VEC], gt[VEC], had[VEC];
+        vector_or<VEC>(p.v.scale, b, f, c, 0.f, up);
+        vadd(up, up, 1.f);
+        vector_or<VEC>(p.v.gate, b, f, c, 1.f, gt);
 #pragma unroll
-          for (int i = 0; i < kSums; ++i)
-            if (p.total_sums >> i & 1)
-              total[i * a.width + c] = (i < 2 ? up : gt) * q[i] + (first_total ? 0.f : total[i * a.width + c]);
-        }
+        for (int i = 0; i < kSums; ++i)
+          if (p.total_sums >> i & 1) {
+            if (first_total) {
+#pragma unroll
+              for (int e = 0; e < VEC; ++e) had[e] = 0.f;
+            } else {
+              any_load<VEC>(total, LVSA_DTYPE_F32, i * a.width + c, had);
+            }
+            if (i < 2) vfma(had, up, q[i], had);
+            else vfma(had, gt, q[i], had);
+            any_store<VEC>(total, LVSA_DTYPE_F32, i * a.width + c, had);
+          }
       }
     }
     first_total = false;
@@ -416,7 +435,8 @@ __global__ void __launch_bounds__(32 * kJoinRows) block_norm_sums_kernel(const _
     for (int i = 1; i < static_cast<int>(blockDim.y); ++i) sum[j] += part[j][i][threadIdx.x];
   if (group >= 0) {
     const int b = group / a.frames;
-    store_group(p.g, b, group - b * a.frames, c, sum);
+    const float q[kSums][1] = {{sum[0]}, {sum[1]}, {sum[2]}, {sum[3]}};
+    store_group<1>(p.g, p.v, b, group - b * a.frames, c, q);
     return;
   }
   if (p.g.dweight) any_store(p.g.dweight, a.next.weight_dtype, c, sum[0]);
@@ -469,6 +489,8 @@ int launch(const LvsaBlockNormGrad& g, const Vectors& v, int64_t* ctas_only, cud
   return cudaGetLastError() == cudaSuccess ? LVSA_OK : LVSA_ERR_CUDA;
 }
 
+inline bool out_vector(const LvsaVectors& v) { return reinterpret_cast<uintptr_t>(v.ptr) % 16 == 0; }
+
 // 8 columns a thread up to 5120 channels, 16 beyond and where rows' own
 // instructions weigh more: the norm alone up to 2048 (126360 x 1536: 287 us with
 // 8, 251 with 16), a join of 1025 to 1536 (131040 x 1536: 437 and 414, with a norm
@@ -484,7 +506,8 @@ int launch_width(const LvsaBlockNormGrad& g, int64_t* ctas, cudaStream_t s) {
     const int st = width <= 8 * 384 ? launch<TS, TB, FORM, 1, 8, 384, 1>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
     if (st != LVSA_OK || width % VEC) return st;
   } else if (width % VEC || !rows_vector<TS, VEC>(g.f.x) || !rows_vector<TB, VEC>(g.f.y) || !rows_vector<TS, VEC>(g.dh) ||
-      !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC)) {
+      !rows_vector<TB, VEC>(g.dn) || !rows_vector<TS, VEC>(g.dx) || !rows_vector<TB, VEC>(g.dy) || !v.aligned(VEC) ||
+      !out_vector(g.dgate) || !out_vector(g.dscale) || !out_vector(g.dshift)) {
     return width <= 8 * 384 ? launch<TS, TB, FORM, 1, 8, 384, 1>(g, v, ctas, s) : launch<TS, TB, FORM, 1, 16, 512, 1>(g, v, ctas, s);
   }
   if constexpr (FORM == 0) {

@@ -213,6 +213,24 @@ __device__ __forceinline__ void any_load(const void* p, int32_t dtype, int64_t i
     }
   }
 }
+// VEC consecutive values to element i, as any_load.
+template <int VEC>
+__device__ __forceinline__ void any_store(void* p, int32_t dtype, int64_t i, const float (&f)[VEC]) {
+  if (dtype == LVSA_DTYPE_F32) {
+    constexpr int E = VEC > 4 ? 4 : VEC;
+#pragma unroll
+    for (int j = 0; j < VEC / E; ++j) {
+      float g[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) g[e] = f[j * E + e];
+      Pack<float, E>::store(static_cast<float*>(p) + i + j * E, g);
+    }
+  } else if (dtype == LVSA_DTYPE_BF16) {
+    Pack<__nv_bfloat16, VEC>::store(static_cast<__nv_bfloat16*>(p) + i, f);
+  } else {
+    Pack<__half, VEC>::store(static_cast<__half*>(p) + i, f);
+  }
+}
 template <int VEC>
 __device__ __forceinline__ void vector_or(const Vector& v, int64_t b, int64_t f, int c, float otherwise, float (&o)[VEC]) {
   if (v.ptr) {
