@@ -61,12 +61,13 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, group: int) -> W4Weight:
     if scales.device != codes.device or tuple(scales.shape) != (n, -(-k // group)):
         raise ValueError(f"pack_w4: scales must be [{n}, {-(-k // group)}] on {codes.device}, got "
                          f"{tuple(scales.shape)} on {scales.device}")
-    codes = codes if codes.stride(1) == 1 and codes.stride(0) >= k else codes.contiguous()
+    if (codes.stride(1) != 1 and k > 1) or (codes.stride(0) < k and n > 1):
+        codes = codes.contiguous()
     lib, size = N.load(), ctypes.c_int64()
     N.check(lib.lvsa_w4_bytes(n, k, ctypes.byref(size)), "lvsa_w4_bytes")
     tiles = torch.empty(size.value, dtype=torch.uint8, device=codes.device)
     with torch.cuda.device(codes.device):
-        st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0), n, k, tiles.data_ptr(),
+        st = lib.lvsa_w4_pack(codes.data_ptr(), codes.stride(0) if n > 1 else k, n, k, tiles.data_ptr(),
                               torch.cuda.current_stream().cuda_stream)
     N.check(st, "lvsa_w4_pack")
     # Two words a tile of 64 columns for group 32, one otherwise; a word has rows r and r + 8.
@@ -121,16 +122,16 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear_w4 has no backward: call it under torch.no_grad() or on detached tensors")
     rows = x if x.dim() == 2 else x.reshape(-1, weight.k)
-    if rows.stride(1) != 1 or rows.stride(0) < weight.k:
+    m = rows.shape[0]
+    if (rows.stride(1) != 1 and weight.k > 1) or (rows.stride(0) < weight.k and m > 1):
         rows = rows.contiguous()
     if bias is not None and bias.stride(0) != 1:
         bias = bias.contiguous()
-    m = rows.shape[0]
     out = torch.empty(m, weight.n, dtype=out_dtype, device=x.device)
     if m:
         launch("lvsa_w4_linear", W4_LINEAR.pack(
             rows.data_ptr(), weight.tiles.data_ptr(), weight.scales.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            out.data_ptr(), rows.stride(0), weight.n, m, weight.n, weight.k, weight.group, _DT[x.dtype],
-            _DT[out_dtype], 0 if bias is None else _DT[bias.dtype], _DT[weight.scales.dtype], _ACT[activation], 0),
-            x.get_device())
+            out.data_ptr(), rows.stride(0) if m > 1 else weight.k, weight.n, m, weight.n, weight.k, weight.group,
+            _DT[x.dtype], _DT[out_dtype], 0 if bias is None else _DT[bias.dtype], _DT[weight.scales.dtype],
+            _ACT[activation], 0), x.get_device())
     return out if x.dim() == 2 else out.view(*x.shape[:-1], weight.n)

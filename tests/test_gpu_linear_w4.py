@@ -116,6 +116,20 @@ def test_shapes_and_strides():
     assert torch.equal(pack_w4(codes.t().contiguous().t(), scales, 64).tiles, w.tiles)
 
 
+def test_one_row_with_any_stride():
+    """A dimension of one element counts as contiguous whatever its stride is."""
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    codes, scales = _make(1, 192, 64, BF, 4)
+    w = pack_w4(codes, scales, 64)
+    assert torch.equal(pack_w4(codes.clone().as_strided((1, 192), (1, 1)), scales, 64).tiles, w.tiles)
+    x = torch.randn(1, 192, device="cuda", dtype=BF)
+    want = linear_w4(x, w)
+    assert torch.equal(linear_w4(x.view(192, 1).t(), w), want)
+    assert torch.equal(linear_w4(x.as_strided((1, 192), (0, 1)), w), want)
+    one = pack_w4(codes[:, :1], scales[:, :1], 64)
+    assert torch.equal(linear_w4(x.view(192, 1).as_strided((192, 1), (1, 7)), one), linear_w4(x.view(192, 1), one))
+
+
 def test_quantize():
     """The nearest code: off by at most half a step, and exactly the codes back from what they stand for."""
     from longvideosparseattention_b200.linear_w4 import linear_w4, quantize_w4
