@@ -35,6 +35,7 @@ namespace {
 
 constexpr int kTileN = 16, kTileK = 64;
 constexpr int kMaxShared = 227 * 1024 - 1024;
+constexpr int kMaxSize = 1 << 30;  // of n and k: indices of columns and rows stay below 2^31, rounded up and past a stretch's end
 // Warps of a CTA, as many as the registers allow, and tiles of a warp on their
 // way.  One row of 30720 x 5120: 28 warps with 4 tiles 18.9 us, with 3 19.4, 5
 // 19.7, 6 19.9; 32 with 4 19.8, with 3 20.3; prefetching further to L2 is slower
@@ -321,6 +322,7 @@ int shared_bytes(int nt, bool halves, int splits, int slots, int chunk, int cols
   return cols * column_pitch(splits * chunk) * 16 + splits * chunk * (halves ? 2 : 1) * 8 * nt * 4 +
          splits * slots * 8 * nt * kTileN * 4;
 }
+constexpr int kMaxHeld = kMaxShared / kTileK;  // k tiles of a column that could fit; keeps the sums above below 2^31
 
 template <int NT, bool HALVES, typename TSc>
 int launch(W4Params p, cudaStream_t s) {
@@ -343,8 +345,8 @@ int launch(W4Params p, cudaStream_t s) {
     // All of x at once where it fits, else a multiple of kAhead tiles of each
     // stretch, which are fewer and longer where even that does not.
     p.chunk = p.stretch;
-    if (shared_of() > kMaxShared) {
-      p.chunk = p.chunk / kAhead * kAhead;
+    if (p.stretch > kMaxHeld || shared_of() > kMaxShared) {
+      p.chunk = std::min(p.chunk, kMaxHeld) / kAhead * kAhead;
       while (p.chunk > kAhead && shared_of() > kMaxShared) p.chunk -= kAhead;
     }
     if (p.chunk > 0 && shared_of() <= kMaxShared) break;
@@ -379,6 +381,7 @@ int launch_group(const W4Params& p, cudaStream_t s) {
 extern "C" int lvsa_w4_bytes(int32_t n, int32_t k, int64_t* bytes) {
   using namespace lvsa;
   if (!bytes || n < 1 || k < 1) return LVSA_ERR_INVALID_ARG;
+  if (n > kMaxSize || k > kMaxSize) return LVSA_ERR_UNSUPPORTED;
   *bytes = (static_cast<int64_t>(n) + kTileN - 1) / kTileN * ((static_cast<int64_t>(k) + kTileK - 1) / kTileK) * 512;
   return LVSA_OK;
 }
@@ -402,8 +405,8 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   if (!a || a->m < 0 || a->n < 1 || a->k < 1) return LVSA_ERR_INVALID_ARG;
   if (a->group != 32 && a->group != 64 && a->group != 128) return LVSA_ERR_UNSUPPORTED;
   if (!known_type(a->x_dtype) || !known_type(a->out_dtype) || (a->bias && !known_type(a->bias_dtype)) ||
-      (a->scale_dtype != LVSA_DTYPE_BF16 && a->scale_dtype != LVSA_DTYPE_F16) || a->n > INT32_MAX - kTileN ||
-      a->k > INT32_MAX - kTileK)
+      (a->scale_dtype != LVSA_DTYPE_BF16 && a->scale_dtype != LVSA_DTYPE_F16) || a->n > kMaxSize || a->k > kMaxSize ||
+      a->m > 65535)  // a pass a block row
     return LVSA_ERR_UNSUPPORTED;
   if (a->activation != LVSA_W4_ACT_NONE && a->activation != LVSA_W4_ACT_SILU) return LVSA_ERR_INVALID_ARG;
   if (!a->tiles || !a->scales || (a->m > 0 && (!a->x || !a->out || a->ldx < a->k || a->ldo < a->n))) return LVSA_ERR_INVALID_ARG;
@@ -414,7 +417,6 @@ extern "C" int lvsa_w4_linear(const LvsaW4Linear* a, void* stream) {
   p.k_tiles = (a->k + kTileK - 1) / kTileK;
   p.row_tiles = (a->n + kTileN - 1) / kTileN;
   p.x_vectors = vector_vector(Vector{a->x, a->ldx, 0, a->x_dtype}, 8);
-  if (a->m > 65535) return LVSA_ERR_UNSUPPORTED;  // a pass a block row
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return a->scale_dtype == LVSA_DTYPE_BF16 ? launch_group<__nv_bfloat16>(p, s) : launch_group<__half>(p, s);
 }

@@ -105,7 +105,7 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     their group; products with codes are exact and sums fp32, with one
     rounding of the result.  A row with an infinity or NaN gives NaN.  Made for
     few rows (a row a sequence or a latent frame): each further 21 read the
-    weights once more.  Inference only: x must not require grad."""
+    weights once more, and 65535 are the most.  Inference only: x must not require grad."""
     if not x.is_cuda:
         raise RuntimeError("linear_w4 needs CUDA tensors (no CPU fallback)")
     out_dtype = x.dtype if out_dtype is None else out_dtype

@@ -161,6 +161,20 @@ def test_offsets_past_32_bits():
         _check(y[:, part], want, size)
 
 
+def test_a_row_of_millions():
+    """Bytes of x as digits pass 32 bits.  Values are powers of two and scales 1:
+    every sum is a whole number below 2^24, and so exact in any order."""
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    m, k = 21, 36_000_065
+    codes = torch.randint(-7, 8, (1, k), device="cuda", dtype=torch.int8)
+    sums = torch.cumsum(codes[0].long(), 0)
+    assert 8 * int(sums.max() - sums.min()) < 2 ** 24
+    w = pack_w4(codes, torch.ones(1, -(-k // 128), device="cuda", dtype=BF), 128)
+    size = torch.tensor([(-1.0) ** i * 2.0 ** (i % 3) for i in range(m)], device="cuda")
+    x = size.to(BF)[:, None].expand(m, k).contiguous()
+    assert torch.equal(linear_w4(x, w, out_dtype=F32)[:, 0], size * sums[-1])
+
+
 def test_infinities_and_large_rows():
     from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
     codes, scales = _make(64, 256, 64, BF, 5)

@@ -51,7 +51,12 @@ def test_checks():
         assert call(_args(**bad)) == N.LVSA_ERR_UNSUPPORTED, bad
     for bad in (dict(tiles=FAKE + 8), dict(scales=FAKE + 4)):
         assert call(_args(**bad)) == N.LVSA_ERR_ALIGNMENT, bad
+    for bad in (dict(n=2 ** 30 + 1, ldo=2 ** 31), dict(k=2 ** 30 + 1, ldx=2 ** 31), dict(m=65536)):
+        assert call(_args(**bad)) == N.LVSA_ERR_UNSUPPORTED, bad
     size = ctypes.c_int64()
+    for n, k in ((2 ** 30 + 1, 1), (1, 2 ** 30 + 1)):
+        assert lib.lvsa_w4_bytes(n, k, ctypes.byref(size)) == N.LVSA_ERR_UNSUPPORTED
+        assert lib.lvsa_w4_pack(FAKE, k, n, k, FAKE, None) == N.LVSA_ERR_UNSUPPORTED
     assert lib.lvsa_w4_bytes(17, 65, ctypes.byref(size)) == N.LVSA_OK and size.value == 2 * 2 * 512
     assert lib.lvsa_w4_bytes(0, 65, ctypes.byref(size)) == N.LVSA_ERR_INVALID_ARG
     assert lib.lvsa_w4_bytes(1, 1, None) == N.LVSA_ERR_INVALID_ARG
