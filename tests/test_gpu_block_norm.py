@@ -219,6 +219,16 @@ def _gradient_sizes(t, norm, post, alpha, seeds, join, eps=1e-6):
     return out
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("shape", [(1, 592, 4, 45), (1, 595, 5, 1155), (2, 310, 2, 2047), (2, 21, 3, 1539), (1, 10, 2, 2049),
+                                   (1, 600, 600, 33), (1, 37, 1, 4097)])
+def test_widths_of_no_vector(shape, form):
+    """On both sides of 592 rows (four an SM) and of 4 values a thread."""
+    types = TYPES[(shape[3] + FORMS.index(form)) % len(TYPES)]
+    test_forward(shape, types, form)
+    test_backward(shape, types, form)
+
+
 def test_gradient_against_differences():
     """Along a direction, central differences of the fp32 kernels themselves:
     off by the step's square (1e-4) and by the outputs' rounding over it."""
