@@ -377,8 +377,9 @@ int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
  *
  * The values of x that one scale goes with count to 2^-22 of their largest;
  * products with codes are exact, sums fp32, with one rounding to the output's
- * type.  A row of x that holds an infinity or NaN gives NaN.  n and k up to
- * 2^30, m up to 65535. */
+ * type.  A row of x that holds an infinity or NaN gives NaN; finite x of any
+ * size gives what its sums in fp32 give, with scales below 2^116.  n and k up
+ * to 2^30, m up to 65535. */
 enum { LVSA_W4_ACT_NONE = 0, LVSA_W4_ACT_SILU = 1 };
 typedef struct LvsaW4Linear {
   const void* x;     /* [m, k], row stride ldx elements, bf16 / f16 / fp32       */

@@ -10,9 +10,11 @@
 // with become whole numbers of 23 bits and sign, their largest 2^21 .. 2^22 by
 // a power of two, in three signed digits of 8 bits: m16n8k32 multiplies them,
 // weights as its 16 rows, digits of rows of x as its 8 columns, without any
-// rounding, and starts from 1.5 2^23 as a float's bits, so that the sum is a
-// float after one subtraction.  Scale, digit's place and power of two join it
-// in fp32.  So x counts to 2^-22 of the largest of its neighbours, as sums in
+// rounding, and starts from 1.5 2^14 as a float's bits, so that the sum over 2^9
+// is a float after one subtraction.  The scale multiplies it first, then digit's
+// place and power of two in fp32: a group's term leaves fp32's range only where
+// its result does (the sum alone times a power near the end of the range would),
+// or where a scale passes 2^116.  So x counts to 2^-22 of the largest of its neighbours, as sums in
 // fp32 count, whatever its type.
 //
 // Work.  A CTA an SM; x, as digits, in its shared memory.  A warp takes a row
@@ -86,8 +88,10 @@ __device__ __forceinline__ void mma(int (&d)[4], const uint32_t (&a)[4], uint32_
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
 }
 constexpr int kDigits = 3;
-constexpr int kMagic = 0x4b400000;  // 1.5 2^23: a sum of at most 64 x 128 x 128 = 2^20 leaves its exponent
-constexpr float kMagicValue = 12582912.f;
+// 1.5 2^14 in steps of 2^-9: a sum of at most 64 x 128 x 128 = 2^20 of them leaves its exponent.
+constexpr int kMagic = 0x46c00000;
+constexpr float kMagicValue = 24576.f;
+constexpr int kRounder = 0x4b400000;  // 1.5 2^23: adding it rounds to a whole number
 
 // NT: column tiles of 8 (digits of rows of x); HALVES: groups of 32 columns.
 template <int NT, bool HALVES, typename TSc>
@@ -140,14 +144,15 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       // Exponents below 26 count as 26: smaller values than 2^-123 are lost.
       const uint32_t power = min(max(most >> 23, 26u), 254u);
       const float down = __uint_as_float((275u - power) << 23);
-      // 2^-16 for the codes' 16; infinities and NaN make the row NaN.
-      float up = most < 0x7f800000u ? __uint_as_float((power - 25u) << 23) : __uint_as_float(0x7fc00000u);
-      // Rounded to a whole number by 1.5 2^23, and with 128 (1 + 256 + 65536)
-      // more, the bytes of it are the digits + 128.
+      // 1 / down, 2^-4 for the codes' 16 and 2^9 for the sums' steps: 2^127 at
+      // most with the last digit's 2^16.  Infinities and NaN make the row NaN.
+      float up = most < 0x7f800000u ? __uint_as_float((power - 16u) << 23) : __uint_as_float(0x7fc00000u);
+      // Rounded to a whole number, and with 128 (1 + 256 + 65536) more, the bytes
+      // of it are the digits + 128.
       uint32_t number[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        number[e] = (__float_as_uint(fmaf(v[e], down, kMagicValue)) - (kMagic - 0x00808080u)) ^ 0x00808080u;
+        number[e] = (__float_as_uint(fmaf(v[e], down, __int_as_float(kRounder))) - (kRounder - 0x00808080u)) ^ 0x00808080u;
 #pragma unroll
       for (int digit = 0; digit < kDigits; ++digit) {
         uint32_t packed[2];
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
                   *reinterpret_cast<const float2*>(x_scale + scale_at + (u * kBlocks + block) * kCols + 8 * (t0 + q));
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                acc[t0 + q][i] += (i < 2 ? lo : hi)[block] * ((__int_as_float(sum[q][i]) - kMagicValue) * (i & 1 ? up.y : up.x));
+                acc[t0 + q][i] += ((i < 2 ? lo : hi)[block] * (__int_as_float(sum[q][i]) - kMagicValue)) * (i & 1 ? up.y : up.x);
             }
           };
 #pragma unroll

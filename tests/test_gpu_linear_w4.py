@@ -276,3 +276,27 @@ def test_block_of_a_layer():
                       (out, definition(h.double(), y2.double(), g2.double())[0])):
         assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -18 * 30).all()
     assert out.shape == x.shape and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 5, 9, 30])
+def test_large_values_of_x(m, group):
+    """Results in fp32's range though x times the codes alone is not; groups that cancel; and large scales."""
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    g = torch.Generator().manual_seed(7)
+    n, k = 48, 256
+    codes = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8)
+    codes[0], codes[1] = 7, -8
+    codes[2, :128], codes[2, 128:] = 7, -7
+    codes[3, 1::2] = 0
+    codes = codes.cuda()
+    for xt, size, scale in ((BF, 2.0 ** 120, 2.0 ** -9), (F32, 3e37, 2.0 ** -8), (F32, 3e38, 2.0 ** -12), (F32, 1.0, 2.0 ** 100)):
+        scales = torch.full((n, k // group), scale).to(BF).cuda()
+        w = pack_w4(codes, scales, group)
+        x = (size * (1 - torch.rand(m, k, generator=g) / 8)).to(xt).cuda()
+        for act in (None, "silu"):
+            want, bound = _want(x, codes, scales, group, None, act)
+            assert want.abs().max() < 3.3e38
+            _check(linear_w4(x, w, activation=act, out_dtype=F32), want, bound)
+        same = linear_w4(torch.full((m, k), size, device="cuda").to(xt), w, out_dtype=F32)
+        assert (same[:, 2] == 0).all()
