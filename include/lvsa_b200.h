@@ -375,7 +375,8 @@ int lvsa_block_norm_bwd(const LvsaBlockNormGrad* args, void* stream);
  * scales (rows r and r + 8 of a tile), G = 2 for group 32 and 1 otherwise (group
  * 128: each scale twice), 0 past the end.
  *
- * The values of x that one scale goes with count to 2^-22 of their largest;
+ * The values of x that one scale goes with count to 2^-22 of their largest
+ * (2^-128 where that is more);
  * products with codes are exact, sums fp32, with one rounding to the output's
  * type.  A row of x that holds an infinity or NaN gives NaN; finite x of any
  * size gives what its sums in fp32 give, with scales below 2^116.  n and k up

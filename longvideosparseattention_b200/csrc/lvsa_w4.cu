@@ -141,8 +141,8 @@ __global__ void __launch_bounds__(32 * kWarpsW4<NT>, 1) w4_linear_kernel(const _
       for (int e = 0; e < 8; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
 #pragma unroll
       for (int w = 1; w < kLanes; w <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, w));
-      // Exponents below 26 count as 26: smaller values than 2^-123 are lost.
-      const uint32_t power = min(max(most >> 23, 26u), 254u);
+      // Exponents below 21 count as 21 (`down` is 2^127 then): values are off by 2^-128.
+      const uint32_t power = min(max(most >> 23, 21u), 254u);
       const float down = __uint_as_float((275u - power) << 23);
       // 1 / down, 2^-4 for the codes' 16 and 2^9 for the sums' steps: 2^127 at
       // most with the last digit's 2^16.  Infinities and NaN make the row NaN.

@@ -102,7 +102,7 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
 
     x, bias and output in bf16, fp16 or fp32; ``activation`` None or "silu",
     in fp32.  Values of act(x) count to 2^-22 of the largest of the 64 (32) in
-    their group; products with codes are exact and sums fp32, with one
+    their group, or to 2^-128 where that is more; products with codes are exact and sums fp32, with one
     rounding of the result.  A row with an infinity or NaN gives NaN; x may have
     any finite size, scales any below 2^116.  Made for
     few rows (a row a sequence or a latent frame): each further 21 read the

@@ -300,3 +300,16 @@ def test_large_values_of_x(m, group):
             _check(linear_w4(x, w, activation=act, out_dtype=F32), want, bound)
         same = linear_w4(torch.full((m, k), size, device="cuda").to(xt), w, out_dtype=F32)
         assert (same[:, 2] == 0).all()
+
+
+def test_small_values_of_x():
+    """Near the low end of fp32's range a value counts to 2^-128 where that is more than 2^-22 of the largest."""
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    codes, _ = _make(32, 128, 64, BF, 8)
+    scales = torch.full((32, 2), 8.0, device="cuda", dtype=BF)
+    w = pack_w4(codes, scales, 64)
+    g = torch.Generator().manual_seed(9)
+    for power in (-100, -106, -110, -116, -120):
+        x = (torch.randn(3, 128, generator=g) * 2.0 ** power).to(BF).cuda()
+        want, bound = _want(x, codes, scales, 64, None, None)
+        _check(linear_w4(x, w, out_dtype=F32), want, bound + 2.0 ** -128 * 8 * codes.double().abs().sum(-1))
