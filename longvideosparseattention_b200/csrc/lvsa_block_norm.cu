@@ -206,6 +206,40 @@ __global__ void __launch_bounds__(kThreads<VEC, FORM>, 1) block_norm_fwd_kernel(
   }
 }
 
+// Shared memory that a CTA may have beside the kernel's own slots and counts.
+constexpr int kSharedLimit = 227 * 1024 - kMaxWarps * static_cast<int>(2 * sizeof(float2) + sizeof(float));
+// What it takes: the vectors held, and each thread's part of the next row.
+template <typename TS, typename TB, int FORM, int VEC, int K>
+constexpr int shared_bytes(int width, int vectors_held, int threads) {
+  return vectors_held * shared_pitch(width) * static_cast<int>(sizeof(float)) +
+         (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + (FORM > 0 ? sizeof(TB) : 0)) : 0);
+}
+constexpr int warps_of_row(int vectors, int k) { return (vectors + 32 * k - 1) / (32 * k); }
+// Accesses of a thread, in quarters of kElems values: the fewest warps of
+// kElems values a thread, then the fewest values; half of kElems where the rows
+// do not fill the device and a row's latency is the time (2 x 77 rows of 2048:
+// 4.5 us with 32 values, 4.2 with 16).
+template <int VEC>
+constexpr int quarters(int vectors, bool few) {
+  constexpr int kMost = kElems / VEC;
+  const int k = few ? 1 : warps_of_row(vectors, warps_of_row(vectors, kMost));
+  return k > kMost * 3 / 4 ? 4 : k > kMost / 2 ? 3 : 2;
+}
+// One team fits a CTA, with its row and vectors, at every width.
+template <typename TS, typename TB, int FORM>
+constexpr bool one_team_fits() {
+  constexpr int VEC = kVec<TS>, kMost = kElems / VEC, kHeld = FORM == 2 ? 4 : FORM == 1 ? 3 : 2;
+  for (int vectors = 1; vectors * VEC <= LVSA_BLOCK_NORM_MAX_WIDTH; ++vectors)
+    for (int few = 0; few < 2; ++few) {
+      const int q = quarters<VEC>(vectors, few), threads = 32 * warps_of_row(vectors, kMost * q / 4);
+      const int bytes = q == 4   ? shared_bytes<TS, TB, FORM, VEC, kMost>(vectors * VEC, kHeld, threads)
+                        : q == 3 ? shared_bytes<TS, TB, FORM, VEC, kMost * 3 / 4>(vectors * VEC, kHeld, threads)
+                                 : shared_bytes<TS, TB, FORM, VEC, kMost / 2>(vectors * VEC, kHeld, threads);
+      if (threads > kThreads<VEC, FORM> || bytes > kSharedLimit) return false;
+    }
+  return true;
+}
+
 // VEC values an access, K accesses a thread.
 template <typename TS, typename TB, int FORM, int VEC, int K>
 int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
@@ -213,16 +247,17 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
   const int vectors = (a.width + VEC - 1) / VEC;
   const int sms = device_sms();
   if (sms < 1) return LVSA_ERR_CUDA;
-  const int warps = (vectors + 32 * K - 1) / (32 * K);
-  // Teams a CTA: one CTA fills an SM, its vectors held once; fewer while SMs
-  // are left over or a group has few rows to share its vectors.
-  int teams = std::max(1, std::min(kThreads<VEC, FORM> / (32 * warps), warps == 1 ? 32 : 15));
-  while (teams > 1 && (rows < static_cast<int64_t>(teams) * sms || a.seq / a.frames < 4 * teams)) --teams;
-  const int threads = 32 * warps * teams;
+  const int warps = warps_of_row(vectors, K);
   constexpr bool JOIN = FORM > 0;
   const int vectors_held = !JOIN ? 2 : a.post.bias ? 4 : 3;
-  const int shared = vectors_held * shared_pitch(a.width) * static_cast<int>(sizeof(float)) +
-                     (VEC > 1 ? threads * K * VEC * static_cast<int>(sizeof(TS) + (JOIN ? sizeof(TB) : 0)) : 0);
+  auto shared_of = [&](int teams) { return shared_bytes<TS, TB, FORM, VEC, K>(a.width, vectors_held, 32 * warps * teams); };
+  // Teams a CTA: one CTA fills an SM, its vectors held once; fewer while SMs
+  // are left over, a group has few rows to share its vectors, or vectors and
+  // rows do not fit (fp32 joins of some 2900 channels and more).
+  int teams = std::max(1, std::min(kThreads<VEC, FORM> / (32 * warps), warps == 1 ? 32 : 15));
+  while (teams > 1 && (rows < static_cast<int64_t>(teams) * sms || a.seq / a.frames < 4 * teams || shared_of(teams) > kSharedLimit))
+    --teams;
+  const int threads = 32 * warps * teams, shared = shared_of(teams);
   auto kern = teams == 1 ? block_norm_fwd_kernel<TS, TB, FORM, VEC, K, true> : block_norm_fwd_kernel<TS, TB, FORM, VEC, K, false>;
   static std::atomic<uint64_t> done[2], last[2];
   const int64_t ctas = resident_ctas(reinterpret_cast<const void*>(kern), threads, shared, done[teams == 1], last[teams == 1]);
@@ -237,20 +272,17 @@ int launch(const LvsaBlockNorm& a, const Vectors& v, cudaStream_t s) {
 template <typename TS, typename TB, int FORM>
 int launch_width(const LvsaBlockNorm& a, cudaStream_t s) {
   constexpr int VEC = kVec<TS>;
+  static_assert(one_team_fits<TS, TB, FORM>(), "");
   const Vectors v(a);
   const bool few = static_cast<int64_t>(a.batch) * a.seq <= 4 * device_sms();
   // Widths, strides or pointers that 16-byte accesses do not fit go value by value.
   if (a.width % VEC == 0 && rows_vector<TS, VEC>(a.x) && rows_vector<TB, VEC>(a.y) && rows_vector<TS, VEC>(a.h) &&
       rows_vector<TB, VEC>(a.n) && v.aligned(VEC)) {
-    // The fewest warps of kElems values a thread, then the fewest values; half
-    // of kElems where the rows do not fill the device and a row's latency is
-    // the time (2 x 77 rows of 2048: 4.5 us with 32 values, 4.2 with 16).
-    const int vectors = a.width / VEC, warps = (vectors * VEC + 32 * kElems - 1) / (32 * kElems);
     constexpr int kMost = kElems / VEC;
-    const int k = few ? 1 : (vectors + 32 * warps - 1) / (32 * warps);
-    return k > kMost * 3 / 4 ? launch<TS, TB, FORM, VEC, kMost>(a, v, s)
-           : k > kMost / 2   ? launch<TS, TB, FORM, VEC, kMost * 3 / 4>(a, v, s)
-                             : launch<TS, TB, FORM, VEC, kMost / 2>(a, v, s);
+    const int q = quarters<VEC>(a.width / VEC, few);
+    return q == 4   ? launch<TS, TB, FORM, VEC, kMost>(a, v, s)
+           : q == 3 ? launch<TS, TB, FORM, VEC, kMost * 3 / 4>(a, v, s)
+                    : launch<TS, TB, FORM, VEC, kMost / 2>(a, v, s);
   }
   // Few rows: as above, and more threads to make a group's vectors (335 x 1155
   // in 5 frames: 18.1 us with 16 values, 9.4 with 4).

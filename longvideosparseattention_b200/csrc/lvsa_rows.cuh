@@ -340,7 +340,7 @@ struct Columns {
   }
 };
 
-__host__ __device__ inline int shared_pitch(int width) { return (width + 7) & ~7; }
+__host__ __device__ constexpr int shared_pitch(int width) { return (width + 7) & ~7; }
 // Vectors of channels in shared memory, `pitch` floats each.  Of 8 values the
 // first and last four lie half a vector apart, so that the lanes of a warp
 // touch consecutive 16 bytes.

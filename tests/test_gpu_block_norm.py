@@ -470,3 +470,22 @@ def test_refusals_on_cuda_tensors():
             call()
     with pytest.raises(RuntimeError):
         norm_modulate(x.cpu())
+
+
+WIDE = [2932, 4096, 4252, 5120, 5124, 6144, 7172, 8192]  # ends of ranges in which fewer teams than threads allow have room
+
+
+@pytest.mark.parametrize("types", [(F32, F32, F32), (F32, BF, F32), (F32, HF, HF), (BF, BF, F32)])
+@pytest.mark.parametrize("width", WIDE)
+def test_many_wide_rows(width, types):
+    """Rows that fill the device with every team a CTA has room for: joins with and without a norm of the branch.
+    A row's sums take 16 additions of pairs a thread and at most 1 + 5 + 4 more; their errors have either sign."""
+    for form in ((None, False, None, 1.0, True), ("layer", True, None, 0.5, True), ("rms", False, "rms", 1.0, True),
+                 ("layer", True, "layer", -0.7, True)):
+        test_forward((1, 1500, 1, width), types, form)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("width", [4096, 5124, 8192])
+def test_steps_of_many_wide_rows(width, form):
+    test_backward((1, 1200, 2, width), (F32, F32, F32), form)
