@@ -7,6 +7,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -18,6 +19,19 @@ W4_LINEAR = struct.Struct("@PPPPPqqiiiiiiiiii")  # the last: the structure's pad
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def dual_level() -> bool:
+    """Whether a level of forward-mode differentiation is entered (without one no tensor is dual)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
+def refuse_tangents(where: str, tensors) -> None:
+    """Raise for a dual tensor of forward-mode differentiation: a kernel called
+    on its values would drop its tangent without a word."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{where} has no forward-mode derivative")
 
 
 def launch(name: str, args, index: int) -> None:

@@ -20,8 +20,9 @@ vector of frame s // (S / F).  Norms: ``"layer"`` (weight and bias optional) or
 ``"rms"`` (weight optional), over C.  Arithmetic and sums are fp32 with one
 rounding of each output; ``n`` is of ``h`` before its rounding.
 
-All three are differentiable in every tensor (once); gradients of vectors are
-fp32 sums in a fixed order, so a step repeats bit for bit.  Calls run on the
+All three are differentiable in every tensor (once, in reverse mode; dual
+tensors of forward mode are refused); gradients of vectors are fp32 sums in a
+fixed order, so a step repeats bit for bit.  Calls run on the
 current stream and can be captured into a CUDA graph, a backward pass with
 them (``torch.autograd.grad``, after a first step outside the capture).
 """
@@ -36,7 +37,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from ._launch import BLOCK_NORM, BLOCK_NORM_GRAD, launch
+from ._launch import BLOCK_NORM, BLOCK_NORM_GRAD, dual_level, launch, refuse_tangents
 
 _DT = {torch.bfloat16: N.LVSA_DTYPE_BF16, torch.float16: N.LVSA_DTYPE_F16, torch.float32: N.LVSA_DTYPE_F32}
 _KINDS = {"layer": N.LVSA_BLOCK_NORM_LAYER, "rms": N.LVSA_BLOCK_NORM_RMS}
@@ -114,6 +115,8 @@ def _channel(where: str, name: str, t: torch.Tensor, C: int, device: int) -> tor
 
 def _run(where, x, y, gate, alpha, post_norm, post_weight, post_bias, post_eps, norm, weight, bias, scale, shift, eps,
          out_dtype):
+    if dual_level():
+        refuse_tangents(where, (x, y, gate, scale, shift, weight, bias, post_weight, post_bias))
     if not x.is_cuda:
         raise RuntimeError(f"{where} needs CUDA tensors (no CPU fallback)")
     dtype, shape, device = x.dtype, x.shape, x.get_device()
@@ -281,6 +284,8 @@ def _workspace(stream: torch.dtype, branch: torch.dtype, B: int, S: int, frames:
 def _backward(ctx, dh, dn):
     if dh is None and dn is None:
         return (None,) * 10
+    if dual_level():
+        refuse_tangents("the block norms' backward", (dh, dn))
     form = ctx.form
     saved = ctx.saved_tensors
     tensors, stats, post_stats = saved[:9], saved[9], saved[10]

@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from ._launch import W4_LINEAR, launch
+from ._launch import W4_LINEAR, dual_level, launch, refuse_tangents
 
 _DT = {torch.bfloat16: N.LVSA_DTYPE_BF16, torch.float16: N.LVSA_DTYPE_F16, torch.float32: N.LVSA_DTYPE_F32}
 _ACT = {None: N.LVSA_W4_ACT_NONE, "silu": N.LVSA_W4_ACT_SILU}
@@ -102,11 +102,14 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
 
     x, bias and output in bf16, fp16 or fp32; ``activation`` None or "silu",
     in fp32.  Values of act(x) count to 2^-22 of the largest of the 64 (32) in
-    their group, or to 2^-128 where that is more; products with codes are exact and sums fp32, with one
-    rounding of the result.  A row with an infinity or NaN gives NaN; x may have
-    any finite size, scales any below 2^116.  Made for
-    few rows (a row a sequence or a latent frame): each further 21 read the
-    weights once more, and 65535 are the most.  Inference only: x must not require grad."""
+    their group, or to 2^-128 where that is more; products with codes are exact
+    and sums fp32, with one rounding of the result.  A row with an infinity or NaN
+    gives NaN; x may have any finite size, scales any below 2^116.  Made for few
+    rows (a row a sequence or a latent frame): each further 21 read the weights
+    once more, and 65535 are the most.  Inference only: x must not require grad
+    or be a dual tensor."""
+    if dual_level():
+        refuse_tangents("linear_w4", (x, bias))
     if not x.is_cuda:
         raise RuntimeError("linear_w4 needs CUDA tensors (no CPU fallback)")
     out_dtype = x.dtype if out_dtype is None else out_dtype

@@ -125,3 +125,20 @@ def test_packed_arguments_have_the_structures_layout():
         values = list(range(1, n + 1))
         got = list(leaves(struct.from_buffer_copy(packer.pack(*values))))
         assert got == values[:len(got)] and n - len(got) in (0, 1)
+
+
+def test_tangents_are_refused():
+    """Where a level of forward-mode differentiation is entered, of dual tensors only."""
+    from torch.autograd import forward_ad
+
+    from longvideosparseattention_b200.block_norm import gate_residual_norm, norm_modulate
+    from longvideosparseattention_b200._launch import refuse_tangents
+    x, v = torch.zeros(1, 2, 8), torch.zeros(8)
+    refuse_tangents("here", (x, None))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(v, torch.ones(8))
+        for call in (lambda: refuse_tangents("here", (x, None, dual)), lambda: norm_modulate(x, scale=dual),
+                     lambda: gate_residual_norm(x, x, dual)):
+            with pytest.raises(NotImplementedError):
+                call()
+        refuse_tangents("here", (x, None, v))

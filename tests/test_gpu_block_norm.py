@@ -489,3 +489,35 @@ def test_many_wide_rows(width, types):
 @pytest.mark.parametrize("width", [4096, 5124, 8192])
 def test_steps_of_many_wide_rows(width, form):
     test_backward((1, 1200, 2, width), (F32, F32, F32), form)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor raises rather than losing its tangent, with and without gradients; so does a transform."""
+    from torch.autograd import forward_ad
+
+    from longvideosparseattention_b200.block_norm import gate_residual, gate_residual_norm, norm_modulate
+    g = torch.Generator().manual_seed(3)
+    x, y, v = _make((1, 4, 64), F32, g), _make((1, 4, 64), F32, g), _make((64,), F32, g)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: norm_modulate(dual(x)), lambda: norm_modulate(x, scale=dual(v)),
+                     lambda: gate_residual(x, dual(y)), lambda: gate_residual(x, y, dual(v)),
+                     lambda: gate_residual_norm(x, y, weight=dual(v)), lambda: gate_residual_norm(x, y, shift=dual(v)),
+                     lambda: gate_residual(x, y, post_norm="layer", post_weight=v, post_bias=dual(v)),
+                     lambda: norm_modulate(x.clone().requires_grad_(True), weight=dual(v))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    call()
+        norm_modulate(x, scale=v)  # none of its tensors is dual
+        z = x.clone().requires_grad_(True)
+        n = norm_modulate(z)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(n, z, dual(y))
+    z = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(norm_modulate(z), z, y[None], is_grads_batched=True)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(norm_modulate, (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(norm_modulate)(x[None])

@@ -313,3 +313,23 @@ def test_small_values_of_x():
         x = (torch.randn(3, 128, generator=g) * 2.0 ** power).to(BF).cuda()
         want, bound = _want(x, codes, scales, 64, None, None)
         _check(linear_w4(x, w, out_dtype=F32), want, bound + 2.0 ** -128 * 8 * codes.double().abs().sum(-1))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor raises rather than losing its tangent, also without gradients; so does a transform."""
+    from torch.autograd import forward_ad
+
+    from longvideosparseattention_b200.linear_w4 import linear_w4, pack_w4
+    codes, scales = _make(32, 64, 64, BF, 6)
+    w = pack_w4(codes, scales, 64)
+    x, bias = torch.randn(2, 64, device="cuda"), torch.randn(32, device="cuda")
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, torch.ones_like(x)), w), (x, w, forward_ad.make_dual(bias, bias))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    linear_w4(*args)
+        linear_w4(x, w, bias)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda v: linear_w4(v, w), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda v: linear_w4(v, w))(x)
