@@ -81,7 +81,8 @@ def pack_w4(codes: torch.Tensor, scales: torch.Tensor, group: int) -> W4Weight:
 
 def quantize_w4(weight: torch.Tensor, group: int = 64, scale_dtype: torch.dtype = torch.bfloat16) -> W4Weight:
     """Round a weight [n, k] to the nearest code -7 .. 7 of its group's scale,
-    the largest size in the group over 7."""
+    the largest size in the group over 7.  Refuses a weight with an infinity or
+    NaN, or too large for ``scale_dtype`` (so it waits for the device once)."""
     if weight.dim() != 2:
         raise ValueError(f"quantize_w4: weight must be [n, k], got {tuple(weight.shape)}")
     if group not in GROUPS:
@@ -91,6 +92,8 @@ def quantize_w4(weight: torch.Tensor, group: int = 64, scale_dtype: torch.dtype 
     n, k = weight.shape
     w = torch.nn.functional.pad(weight.detach().float(), (0, -k % group)).unflatten(1, (-1, group))
     scales = (w.abs().amax(-1) / 7).to(scale_dtype)
+    if not torch.isfinite(scales).all():  # NaN and infinities of the weight among them
+        raise ValueError(f"quantize_w4: weight has values that are not finite, or whose scale passes {scale_dtype}")
     step = scales.float()[..., None]
     codes = torch.where(step > 0, w / step, 0.0).round_().clamp_(-7, 7).to(torch.int8).flatten(1)[:, :k]
     return pack_w4(codes, scales, group)

@@ -71,3 +71,16 @@ def test_cpu_tensors_are_refused():
         pack_w4(torch.zeros(4, 64, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.bfloat16), 64)
     with pytest.raises(RuntimeError):
         quantize_w4(torch.zeros(4, 64))
+
+
+def test_quantize_refuses_what_has_no_codes():
+    """An infinity or NaN anywhere, or a scale past its type: before any kernel runs."""
+    from longvideosparseattention_b200.linear_w4 import quantize_w4
+    for bad, dtype in ((float("inf"), torch.bfloat16), (float("-inf"), torch.float16), (float("nan"), torch.bfloat16),
+                       (1e6, torch.float16)):
+        weight = torch.ones(3, 100)
+        weight[2, 99] = bad
+        with pytest.raises(ValueError):
+            quantize_w4(weight, 32, dtype)
+    with pytest.raises(ValueError):
+        quantize_w4(torch.full((1, 64), 1e300, dtype=torch.float64))
