@@ -340,7 +340,7 @@ typedef struct LvsaBlockNorm {
   float residual_scale;
   int32_t stream_dtype, branch_dtype, batch, seq, frames, width;
   float* stats;      /* [batch * seq][2] mean and 1 / deviation of next, for the backward; or NULL */
-  float* post_stats; /* the same of post */
+  float* post_stats; /* the same of post; both 8-byte aligned */
 } LvsaBlockNorm;
 int lvsa_block_norm_fwd(const LvsaBlockNorm* args, void* stream);
 

@@ -557,6 +557,8 @@ inline int check_block_norm(const LvsaBlockNorm& a) {
   if (!a.x.ptr || (!a.y.ptr && !a.n.ptr)) return LVSA_ERR_INVALID_ARG;
   if (a.batch < 0 || a.seq < 0 || a.frames < 1 || a.width < 1) return LVSA_ERR_INVALID_ARG;
   if (a.seq % a.frames) return LVSA_ERR_GEOMETRY;
+  // A row's two statistics are one access.
+  if ((reinterpret_cast<uintptr_t>(a.stats) | reinterpret_cast<uintptr_t>(a.post_stats)) & 7) return LVSA_ERR_ALIGNMENT;
   if (!known_type(a.stream_dtype) || !known_type(a.branch_dtype) || a.width > LVSA_BLOCK_NORM_MAX_WIDTH ||
       (a.stream_dtype != a.branch_dtype && a.stream_dtype != LVSA_DTYPE_F32) ||
       static_cast<int64_t>(a.batch) * a.seq > LVSA_BLOCK_NORM_MAX_ROWS)

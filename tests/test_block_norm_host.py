@@ -142,3 +142,17 @@ def test_tangents_are_refused():
             with pytest.raises(NotImplementedError):
                 call()
         refuse_tangents("here", (x, None, v))
+
+
+def test_statistics_are_aligned():
+    """A row's pair of statistics is one 8-byte access: a pointer between them is refused, with no rows too."""
+    lib = N.load()
+    rows = N.LvsaRows(FAKE, 0, 64)
+    for where in ("stats", "post_stats"):
+        kw = dict(stats=FAKE, post_stats=FAKE, post=N.LvsaRowNorm(2, 0.0))
+        assert _fwd(_args(**kw)) == N.LVSA_OK
+        kw[where] = FAKE + 4
+        assert _fwd(_args(**kw)) == N.LVSA_ERR_ALIGNMENT
+        g = N.LvsaBlockNormGrad()
+        g.f, g.dn = _args(**kw), rows
+        assert lib.lvsa_block_norm_bwd(ctypes.byref(g), None) == N.LVSA_ERR_ALIGNMENT
