@@ -32,13 +32,28 @@ GROUPS = (32, 64, 128)
 
 @dataclass(frozen=True)
 class W4Weight:
-    """A [n, k] weight laid out for ``linear_w4`` (made by ``pack_w4``)."""
+    """A [n, k] weight laid out for ``linear_w4`` (made by ``pack_w4``): the
+    kernel reads ``tiles`` and ``scales`` by n, k and group, which have to fit.
+    Its tensors may be kept and moved like others and put together again."""
 
     n: int
     k: int
     group: int
     tiles: torch.Tensor   # uint8
     scales: torch.Tensor  # bf16 / fp16
+
+    def __post_init__(self):
+        if self.group not in GROUPS or self.n < 1 or self.k < 1:
+            raise ValueError(f"W4Weight: [{self.n}, {self.k}] in groups of {self.group}: sizes from 1 and groups of {GROUPS} expected")
+        if self.tiles.dtype != torch.uint8 or self.scales.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"W4Weight: uint8 tiles and bf16 / fp16 scales expected, got {self.tiles.dtype} and {self.scales.dtype}")
+        tiles = -(-self.n // 16) * -(-self.k // 64)
+        want = (tiles * 512, tiles * 16 * max(1, 64 // self.group))
+        if (self.tiles.numel(), self.scales.numel()) != want or not (self.tiles.is_contiguous() and self.scales.is_contiguous()):
+            raise ValueError(f"W4Weight: [{self.n}, {self.k}] in groups of {self.group} has {want[0]} bytes of tiles and "
+                             f"{want[1]} scales, contiguous; got {self.tiles.numel()} and {self.scales.numel()}")
+        if self.tiles.device != self.scales.device:
+            raise ValueError(f"W4Weight: tiles on {self.tiles.device}, scales on {self.scales.device}")
 
     @property
     def device(self) -> torch.device:

@@ -84,3 +84,24 @@ def test_quantize_refuses_what_has_no_codes():
             quantize_w4(weight, 32, dtype)
     with pytest.raises(ValueError):
         quantize_w4(torch.full((1, 64), 1e300, dtype=torch.float64))
+
+
+def test_weights_that_do_not_fit_their_sizes_are_refused():
+    """The kernel goes by n, k and group: tensors of other sizes would be read out of range."""
+    import dataclasses
+
+    from longvideosparseattention_b200.linear_w4 import W4Weight
+    BF = torch.bfloat16
+
+    def make(n, k, group, tiles, scales, dtype=torch.uint8, sdtype=BF, device="cpu"):
+        return W4Weight(n, k, group, torch.zeros(tiles, dtype=dtype), torch.zeros(scales, dtype=sdtype, device=device))
+    for n, k, group, tiles, scales in ((16, 64, 64, 512, 16), (17, 65, 32, 2048, 128), (1, 200, 128, 2048, 64)):
+        w = make(n, k, group, tiles, scales)
+        for bad in (dict(n=n + 16), dict(k=k + 64), dict(group=32 if group > 32 else 64), dict(n=0), dict(k=-1), dict(group=16),
+                    dict(tiles=w.tiles[1:]), dict(scales=w.scales[1:]), dict(tiles=torch.zeros(2 * tiles, dtype=torch.uint8)[::2]),
+                    dict(scales=torch.zeros(scales, dtype=BF, device="meta"))):
+            with pytest.raises(ValueError):
+                dataclasses.replace(w, **bad)
+        for bad in (dict(tiles=w.tiles.to(torch.int32)), dict(scales=w.scales.float())):
+            with pytest.raises(TypeError):
+                dataclasses.replace(w, **bad)
