@@ -313,7 +313,8 @@ int lvsa_copy_segments(const LvsaCopySegment* segs, int32_t n, int32_t row_bytes
  * only has a bias); post may be LVSA_BLOCK_NORM_NONE.  gate, scale and shift
  * are [batch, frames, width] (NULL: 1, 0 and 0), seq / frames consecutive
  * tokens to each frame; a stride of 0 shares a vector.  fp32 arithmetic, one
- * rounding of each output; n is of h before its rounding. */
+ * rounding of each output; n is of h before its rounding.  Outputs may not
+ * overlap inputs or one another (h may not be x), in the gradients' call either. */
 enum { LVSA_BLOCK_NORM_NONE = 0, LVSA_BLOCK_NORM_LAYER = 1, LVSA_BLOCK_NORM_RMS = 2 };
 #define LVSA_BLOCK_NORM_MAX_WIDTH 8192
 #define LVSA_BLOCK_NORM_MAX_ROWS 2147483000 /* batch * seq */
@@ -387,7 +388,7 @@ typedef struct LvsaW4Linear {
   const void* tiles; /* from lvsa_w4_pack, 16-byte aligned                       */
   const void* scales; /* 8-byte aligned                                          */
   const void* bias;  /* [n] or NULL                                              */
-  void* out;         /* [m, n], row stride ldo elements                          */
+  void* out;         /* [m, n], row stride ldo elements; no overlap with inputs  */
   int64_t ldx, ldo;
   int32_t m, n, k, group; /* group 32, 64 or 128                                 */
   int32_t x_dtype, out_dtype, bias_dtype, scale_dtype; /* scales bf16 or f16     */

@@ -24,7 +24,8 @@ All three are differentiable in every tensor (once, in reverse mode; dual
 tensors of forward mode are refused); gradients of vectors are fp32 sums in a
 fixed order, so a step repeats bit for bit.  Calls run on the
 current stream and can be captured into a CUDA graph, a backward pass with
-them (``torch.autograd.grad``, after a first step outside the capture).
+them (``torch.autograd.grad``, after a first step outside the capture whose
+autograd graph is gone: torch would have the capture wait for its stream).
 """
 
 from __future__ import annotations

@@ -13,7 +13,9 @@
 // As soon as a row's values are taken from it, a thread's slot of shared
 // memory is filled with its part of the team's next row (cp.async), so that
 // every warp has a row on its way at all times without registers for it.
-// Bound: HBM (x and y read once, h and n written once).
+// Bound: HBM (x and y read once, h and n written once): 126360 x 1536 norm alone
+// 94 % of a copy's rate, joins 84 to 93 % up to 8192 channels in fp32 (16380 x 4096
+// 187 us, x 8192 384 us), with a norm of the branch 58 to 85 %.
 #include <algorithm>
 #include <atomic>
 

@@ -17,10 +17,12 @@
 // its last), as do the sums over groups (one row a CTA), and a second kernel
 // adds these in the order of the CTAs.
 // Bound: HBM (x, y, dn, dh read once, dx, dy written once): 90 to 95 % of a copy's
-// rate with a join at 2048 channels or an fp32 stream of 5120.  A norm of the
-// branch adds a second round of sums a row, which waits for the first (66 % at
-// 5120 channels; joining the two rounds into one of ten sums took longer yet, 1590
-// to 2237 us at 70200 rows, for its instructions).
+// rate for 77910 x 2048 with a join and norm and for the norm alone of an fp32
+// stream of 32760 x 5120 (a join alone of the latter in 21 frames: 378 us, 81 %).
+// A norm of the branch adds a second round of sums a row, which waits for the
+// first: 70200 x 5120 in fp32 with 16-bit branches 1490 us, 66 %; 17550 x 5120 in
+// 13 frames 412 us, 60 % (joining the two rounds into one of ten sums took 2237 us
+// at 70200 rows, for its instructions).
 #pragma once
 #include <algorithm>
 #include <atomic>

@@ -28,7 +28,7 @@ __device__ __forceinline__ T from_f(float v) {
   else return v;
 }
 
-// Storage of VEC values of a type: 1, 8 or 16 bytes (fp32 takes at most 4 values).
+// Storage of VEC values of a type: 2, 4, 8 or 16 bytes (fp32 takes at most 4 values).
 template <int BYTES>
 struct Raw;
 template <>

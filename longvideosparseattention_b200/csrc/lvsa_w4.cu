@@ -7,15 +7,17 @@
 // its bytes are one AND, and one shift and AND, away (the integer pipe bounds
 // this kernel next to HBM: f16 weights took 36 operations a tile of 16 x 64,
 // these take 12).  The 64 (32) values of x that one scale of the weights goes
-// with become whole numbers of 23 bits and sign, their largest 2^21 .. 2^22 by
+// with become whole numbers of 22 bits and sign, their largest 2^21 .. 2^22 by
 // a power of two, in three signed digits of 8 bits: m16n8k32 multiplies them,
 // weights as its 16 rows, digits of rows of x as its 8 columns, without any
 // rounding, and starts from 1.5 2^14 as a float's bits, so that the sum over 2^9
 // is a float after one subtraction.  The scale multiplies it first, then digit's
 // place and power of two in fp32: a group's term leaves fp32's range only where
 // its result does (the sum alone times a power near the end of the range would),
-// or where a scale passes 2^116.  So x counts to 2^-22 of the largest of its neighbours, as sums in
-// fp32 count, whatever its type.
+// or where a scale passes 2^116.  So x counts to 2^-22 of the largest of its
+// neighbours, whatever its type, as the terms of a sum in fp32 count beside the
+// largest of them; where that neighbour meets a code of 0, products in fp32 would
+// keep more (a fourth digit would be a third more columns).
 //
 // Work.  A CTA an SM; x, as digits, in its shared memory.  A warp takes a row
 // of tiles (16 rows of weights), or one of `splits` stretches of

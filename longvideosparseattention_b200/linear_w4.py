@@ -3,15 +3,17 @@ few rows: the Linears whose time is that of reading their weights.
 
 In a diffusion transformer these are the ones that the time embedding passes
 through, with one row a sequence or a latent frame: the shift, scale and gate
-vectors of every block (``block_norm``) come from a Linear of SiLU(embedding)
-whose weights are a large part of the model.  An addition of this package: the
-reference leaves them to the model.
+vectors (``block_norm``) come from a Linear of SiLU(embedding), one in every
+block of the HunyuanVideo and CogVideoX models, whose weights are a large part
+of the model, one a step in Wan, whose blocks add a table of their own.  An
+addition of this package: the reference leaves them to the model.
 
     w = quantize_w4(block.modulation.weight)               # once
     shift, scale, gate = linear_w4(temb, w, bias, "silu").chunk(3, dim=-1)
 
 W[n, k] is approximated by scale[n, k // group] * code[n, k], codes -8 .. 7;
-``pack_w4`` takes codes and scales of another quantiser.
+``pack_w4`` takes codes and scales of another quantiser; codes are signed, about
+zero (a checkpoint with zero points has no form here).
 """
 
 from __future__ import annotations
@@ -120,7 +122,8 @@ def linear_w4(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
 
     x, bias and output in bf16, fp16 or fp32; ``activation`` None or "silu",
     in fp32.  Values of act(x) count to 2^-22 of the largest of the 64 (32) in
-    their group, or to 2^-128 where that is more; products with codes are exact
+    their group, whatever codes that one meets, or to 2^-128 where that is more;
+    SiLU of values below -87 is zero; products with codes are exact
     and sums fp32, with one rounding of the result.  A row with an infinity or NaN
     gives NaN; x may have any finite size, scales any below 2^116.  Made for few
     rows (a row a sequence or a latent frame): each further 21 read the weights
